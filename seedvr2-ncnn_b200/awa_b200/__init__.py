@@ -902,3 +902,8 @@ __all__ = ["AwaPlan", "AwaComm", "AwaError", "PlanInfo", "library", "make_window
            "graph_make_dynamic", "manifest_validate", "sha256", "sha256_file", "AwaStack", "StackGraph", "StackIO",
            "AWA_STACK_BEFORE", "AWA_STACK_AFTER", "AWA_F32", "AWA_BF16", "AWA_PREC_FP32", "AWA_PREC_BF16",
            "AWA_BRANCH_VIDEO", "AWA_BRANCH_TEXT"]
+
+
+# The paged key/value cache (include/awa_cache.h) has a module of its own.
+from .cache import (AWA_CACHE_BAD_COORD, AWA_CACHE_BAD_PAGE, AWA_CACHE_GROUP, AWA_INT4, CACHE_SYMBOLS,  # noqa: E402,F401
+                    CacheBatch, CacheRope, KvCache, rope_table)

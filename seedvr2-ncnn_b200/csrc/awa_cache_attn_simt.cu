@@ -1,0 +1,388 @@
+// awa_cache_attn_simt.cu -- attention over the paged key/value cache in fp32
+// arithmetic, for fp32 caches and for head sizes without a tensor-core kernel.
+//
+// out = softmax(scale q K^T) V in one pass over the keys a tile of query rows
+// sees: per block of 64 keys, S = Q K^T in registers, the running maximum m and
+// sum l of each row (base 2, scale folded into the exponent), O = O 2^(m - m')
+// + P V.
+#include "awa_cache_device.cuh"
+#include "awa_rows.cuh"
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+#include <type_traits>
+
+namespace awa
+{
+namespace
+{
+
+namespace cg = cooperative_groups;
+using bf16 = __nv_bfloat16;
+
+constexpr int kThreads = 256;
+constexpr int kKeys = 64;
+constexpr int kPad = 4;  // floats: rows start 4 banks apart, so 16-byte reads of 8 rows do not collide
+
+__host__ __device__ constexpr int shared_floats(int rows, int d)
+{
+    return (rows + 2 * kKeys) * (d + kPad) + rows * (kKeys + kPad);
+}
+
+__device__ __forceinline__ float dot4(float4 a, float4 b, float acc)
+{
+    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, acc))));
+}
+
+// 8 features of one cached row as floats.
+template <int ST>
+__device__ __forceinline__ void cached8(const char* row, const char* params, int f, float (&v)[8])
+{
+    if (ST == AWA_F32)
+        load8(reinterpret_cast<const float*>(row) + f, v);
+    else if (ST == AWA_BF16)
+        load8(reinterpret_cast<const bf16*>(row) + f, v);
+    else
+    {
+        const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(row + f / 2));
+        const uint32_t p = __ldg(reinterpret_cast<const uint32_t*>(params) + f / AWA_CACHE_GROUP);
+        const float scale = __uint_as_float(p << 16), minimum = __uint_as_float(p & 0xffff0000u);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            v[i] = fmaf((float)((codes >> (4 * i)) & 15u), scale, minimum);
+    }
+}
+
+// A block (of a cluster of gridDim.x / tiles that share the keys) takes one
+// tile of R * 16 query rows of one key/value head. Thread (ty, tx) of 16 x 16:
+// rows ty * R + i, keys tx + 16 j, output features 4 (tx + 16 j).
+template <int ST, int R>
+__global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAttnArgs a, int cluster_size)
+{
+    using T = typename std::conditional<ST == AWA_F32, float, bf16>::type;  // of q and out
+    constexpr int kRows = 16 * R;
+    extern __shared__ float4 shared4[];
+    __shared__ QueryTile tile_s;
+    const CacheMemory& mem = a.mem;
+    const int d = mem.head_dim, pitch = d + kPad;
+    float* sq = reinterpret_cast<float*>(shared4);
+    float* sk = sq + kRows * pitch;
+    float* sv = sk + kKeys * pitch;
+    float* sp = sv + kKeys * pitch;
+    const int rank = blockIdx.x % cluster_size;
+    if (threadIdx.x < 32)
+    {
+        const QueryTile t =
+            find_tile(mem, a.batch, a.group, kRows, blockIdx.x / cluster_size, rank == 0 ? a.error_flag : nullptr);
+        if (threadIdx.x == 0)
+            tile_s = t;
+    }
+    __syncthreads();
+    const QueryTile t = tile_s;
+    if (t.b < 0)
+        return;  // the whole cluster
+    const int kv = blockIdx.y;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int chunks = d / 8;
+
+    const T* q = static_cast<const T*>(a.q);
+    for (int i = threadIdx.x; i < kRows * chunks; i += kThreads)
+    {
+        const int r = i / chunks, f = (i - r * chunks) * 8;
+        float v[8] = {};
+        if (r < t.count)
+        {
+            const int m = t.m0 + r;
+            load8(q + (int64_t)(t.row0 + m / a.group) * a.q_stride + (int64_t)(kv * a.group + m % a.group) * d + f, v);
+        }
+        store8(sq + r * pitch + f, v);
+    }
+
+    RowSpan span[R];
+#pragma unroll
+    for (int i = 0; i < R; i++)
+    {
+        const int m = min(ty * R + i, t.count - 1);
+        span[i] = row_span(t.past + (t.m0 + m) / a.group, t.length, a.sinks, a.window, a.frame_tokens);
+    }
+    const RowSpan first = row_span(t.past + t.m0 / a.group, t.length, a.sinks, a.window, a.frame_tokens);
+    const RowSpan last =
+        row_span(t.past + (t.m0 + t.count - 1) / a.group, t.length, a.sinks, a.window, a.frame_tokens);
+    const KeyBlocks blocks = key_blocks(first, last, a.sinks, kKeys);
+
+    const float to_log2 = a.scale * 1.44269504088896341f;
+    float mx[R], sum[R], o[R][2][4];
+#pragma unroll
+    for (int i = 0; i < R; i++)
+    {
+        mx[i] = -INFINITY;
+        sum[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            o[i][j / 4][j % 4] = 0.f;
+    }
+
+    for (int n = rank; n < blocks.count; n += cluster_size)
+    {
+        const int key0 = (n < blocks.prefix ? n : n + blocks.shift) * kKeys;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kKeys * chunks; i += kThreads)
+        {
+            const int r = i / chunks, f = (i - r * chunks) * 8;
+            const int key = key0 + r;
+            float k8[8] = {}, v8[8] = {};
+            // only what some row sees is read: pages outside may be gone
+            if (key < last.hi && (key >= first.lo || key < a.sinks))
+            {
+                const int page = page_of(mem, a.batch, t.b, key, a.error_flag);
+                if (page >= 0)
+                {
+                    const int slot = key & ((1 << mem.page_shift) - 1);
+                    const int row_bytes = ST == AWA_INT4 ? d / 2 : d * (ST == AWA_F32 ? 4 : 2);
+                    const int64_t at = page * mem.page_stride + kv * mem.head_stride + (int64_t)slot * row_bytes;
+                    const int64_t par = page * mem.params_page_stride + kv * mem.params_head_stride +
+                                        (int64_t)slot * (d / AWA_CACHE_GROUP) * 4;
+                    cached8<ST>(mem.k + at, mem.k_params + par, f, k8);
+                    cached8<ST>(mem.v + at, mem.v_params + par, f, v8);
+                }
+            }
+            store8(sk + r * pitch + f, k8);
+            store8(sv + r * pitch + f, v8);
+        }
+        __syncthreads();
+
+        float s[R][4];
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                s[i][j] = 0.f;
+#pragma unroll 4
+        for (int f = 0; f < d; f += 4)
+        {
+            float4 qv[R], kk[4];
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                qv[i] = *reinterpret_cast<const float4*>(sq + (ty * R + i) * pitch + f);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                kk[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * pitch + f);
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    s[i][j] = dot4(qv[i], kk[j], s[i][j]);
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++)
+        {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+            {
+                const int key = key0 + tx + 16 * j;
+                const bool seen = key < span[i].hi && (key >= span[i].lo || key < a.sinks);
+                s[i][j] = seen ? s[i][j] * to_log2 : -INFINITY;
+                top = fmaxf(top, s[i][j]);
+            }
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            top = fmaxf(top, mx[i]);
+            const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: all exponentials 0
+            const float old = fast_exp2(mx[i] - base);
+            mx[i] = top;
+            float part = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+            {
+                const float p = fast_exp2(s[i][j] - base);
+                part += p;
+                sp[(ty * R + i) * (kKeys + kPad) + tx + 16 * j] = p;
+            }
+            sum[i] = sum[i] * old + part;  // of this thread's keys; added up over tx at the end
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                o[i][j / 4][j % 4] *= old;
+        }
+        __syncwarp();  // a row's probabilities come from its own half warp
+#pragma unroll 2
+        for (int key = 0; key < kKeys; key += 4)
+        {
+            float4 p[R];
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                p[i] = *reinterpret_cast<const float4*>(sp + (ty * R + i) * (kKeys + kPad) + key);
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+            {
+                const int f = 4 * (tx + 16 * j);
+                if (f >= d)
+                    break;
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                {
+                    const float4 v = *reinterpret_cast<const float4*>(sv + (key + u) * pitch + f);
+#pragma unroll
+                    for (int i = 0; i < R; i++)
+                    {
+                        const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
+                        o[i][j][0] = fmaf(w, v.x, o[i][j][0]);
+                        o[i][j][1] = fmaf(w, v.y, o[i][j][1]);
+                        o[i][j][2] = fmaf(w, v.z, o[i][j][2]);
+                        o[i][j][3] = fmaf(w, v.w, o[i][j][3]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1)
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], off);
+
+    T* out = static_cast<T*>(a.out);
+    if (cluster_size == 1)
+    {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+        {
+            const int r = ty * R + i;
+            if (r >= t.count)
+                continue;
+            const int m = t.m0 + r;
+            const float inv = sum[i] > 0.f ? 1.f / sum[i] : sum[i] == 0.f ? 0.f : sum[i];
+            T* dst = out + (int64_t)(t.row0 + m / a.group) * a.out_stride + (int64_t)(kv * a.group + m % a.group) * d;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (4 * (tx + 16 * j) < d)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        store1(dst + 4 * (tx + 16 * j) + c, o[i][j][c] * inv);
+        }
+        return;
+    }
+
+    // The cluster's parts meet in shared memory: O, m and l of every block,
+    // joined in the order of the ranks, each block taking a share of the rows.
+    cg::cluster_group cluster = cg::this_cluster();
+    __syncthreads();
+    float* part_o = sq;                // [kRows][pitch]
+    float2* part_ml = reinterpret_cast<float2*>(sk);
+#pragma unroll
+    for (int i = 0; i < R; i++)
+    {
+        const int r = ty * R + i;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            if (4 * (tx + 16 * j) < d)
+                *reinterpret_cast<float4*>(part_o + r * pitch + 4 * (tx + 16 * j)) =
+                    make_float4(o[i][j][0], o[i][j][1], o[i][j][2], o[i][j][3]);
+        if (tx == 0)
+            part_ml[r] = make_float2(mx[i], sum[i]);
+    }
+    cluster.sync();
+    for (int i = rank * kThreads + threadIdx.x; i < t.count * (d / 4); i += cluster_size * kThreads)
+    {
+        const int r = i / (d / 4), f = (i - r * (d / 4)) * 4;
+        float top = -INFINITY;
+        for (int c = 0; c < cluster_size; c++)
+            top = fmaxf(top, cluster.map_shared_rank(part_ml, c)[r].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        float total = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < cluster_size; c++)
+        {
+            const float2 ml = cluster.map_shared_rank(part_ml, c)[r];
+            const float w = fast_exp2(ml.x - base);
+            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part_o, c) + r * pitch + f);
+            total = fmaf(ml.y, w, total);
+            acc.x = fmaf(x.x, w, acc.x);
+            acc.y = fmaf(x.y, w, acc.y);
+            acc.z = fmaf(x.z, w, acc.z);
+            acc.w = fmaf(x.w, w, acc.w);
+        }
+        const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+        const int m = t.m0 + r;
+        T* dst = out + (int64_t)(t.row0 + m / a.group) * a.out_stride + (int64_t)(kv * a.group + m % a.group) * d + f;
+        store1(dst, acc.x * inv);
+        store1(dst + 1, acc.y * inv);
+        store1(dst + 2, acc.z * inv);
+        store1(dst + 3, acc.w * inv);
+    }
+    cluster.sync();  // a block's shared memory stays until every peer has read it
+}
+
+template <int ST, int R>
+int run(const CacheAttnArgs& a, cudaStream_t stream)
+{
+    const int d = a.mem.head_dim;
+    const int64_t tiles = (int64_t)a.batch.rows * a.group / (16 * R) + a.batch.sequences;
+    // Blocks that share a tile's keys: enough to fill the GPU, at most 8 (the
+    // portable cluster size), each with at least two blocks of keys where the
+    // page table's width says how many there can be.
+    const int64_t most = (((int64_t)a.batch.table_width << a.mem.page_shift) + kKeys - 1) / kKeys;
+    int cluster = 1;
+    while (cluster < 8 && tiles * a.mem.heads * cluster < 2 * 148 && most >= 4 * cluster)
+        cluster *= 2;
+    if (tiles * cluster > 0x7fffffff)
+        return (int)cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(tiles * cluster), (unsigned)a.mem.heads);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = shared_floats(16 * R, d) * sizeof(float);
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&config, cache_attention_simt_kernel<ST, R>, a, cluster);
+}
+
+template <int ST>
+int run(const CacheAttnArgs& a, int max_rows, cudaStream_t stream)
+{
+    // 64 rows a tile use the FMA units best; up to 16 rows of a head group,
+    // a tile of 16 does a quarter of the work
+    return (int64_t)max_rows * a.group <= 16 ? run<ST, 1>(a, stream) : run<ST, 4>(a, stream);
+}
+
+}  // namespace
+
+int launch_cache_attention_simt(const CacheAttnArgs& a, int max_rows, cudaStream_t stream)
+{
+    ProfileScope scope("awa_cache_attention_simt", stream);
+    switch (a.mem.storage)
+    {
+    case AWA_F32: return run<AWA_F32>(a, max_rows, stream);
+    case AWA_BF16: return run<AWA_BF16>(a, max_rows, stream);
+    default: return run<AWA_INT4>(a, max_rows, stream);
+    }
+}
+
+int prepare_cache_attention_simt()
+{
+    const auto set = [](const void* kernel, int rows) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    shared_floats(rows, kMaxHeadDim) * (int)sizeof(float));
+    };
+    const void* kernels[3][2] = {
+        {(const void*)cache_attention_simt_kernel<AWA_F32, 1>, (const void*)cache_attention_simt_kernel<AWA_F32, 4>},
+        {(const void*)cache_attention_simt_kernel<AWA_BF16, 1>, (const void*)cache_attention_simt_kernel<AWA_BF16, 4>},
+        {(const void*)cache_attention_simt_kernel<AWA_INT4, 1>, (const void*)cache_attention_simt_kernel<AWA_INT4, 4>}};
+    for (auto& pair : kernels)
+        for (int r = 0; r < 2; r++)
+        {
+            const cudaError_t err = set(pair[r], r ? 64 : 16);
+            if (err != cudaSuccess)
+                return (int)err;
+        }
+    return 0;
+}
+
+}  // namespace awa

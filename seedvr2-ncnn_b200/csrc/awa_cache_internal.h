@@ -1,0 +1,91 @@
+// awa_cache_internal.h -- what the host side of the key/value cache
+// (awa_cache.cpp) hands to its kernels (awa_cache_*.cu).
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+#include "awa_cache.h"
+#include "awa_internal.h"
+
+namespace awa
+{
+
+// The cache's memory as the kernels address it. Strides in bytes.
+struct CacheMemory
+{
+    int storage;
+    int heads;
+    int head_dim;
+    int page_shift;  // log2(page_tokens)
+    int pages;
+    char* k;
+    char* v;
+    int64_t page_stride, head_stride;
+    char* k_params;
+    char* v_params;
+    int64_t params_page_stride, params_head_stride;
+};
+
+struct CacheBatch
+{
+    int sequences;
+    int rows;
+    const int* row_starts;
+    const int* past;
+    const int* page_table;
+    int table_width;
+    int64_t table_stride;
+};
+
+struct CacheAppendArgs
+{
+    CacheMemory mem;
+    CacheBatch batch;
+    int q_heads;  // 0: no q
+    const char *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride;  // elements
+    char* q_out;
+    int64_t q_out_stride;
+    const float2* table;  // NULL: no rotation
+    int max_coord, axes, pairs;
+    const int* coords;
+    int aligned;  // every row can be read and written in 16-byte pieces
+    int* error_flag;
+};
+
+struct CacheReadArgs
+{
+    CacheMemory mem;
+    CacheBatch batch;
+    char *k_out, *v_out;
+    int64_t k_stride, v_stride;  // elements
+    int aligned;
+    int* error_flag;
+};
+
+struct CacheAttnArgs
+{
+    CacheMemory mem;
+    CacheBatch batch;
+    int group;  // q heads per key/value head
+    const void* q;
+    int64_t q_stride;  // elements
+    void* out;
+    int64_t out_stride;
+    float scale;
+    int sinks, window, frame_tokens;
+    int* error_flag;
+};
+
+int launch_cache_append(const CacheAppendArgs& args, int in_dtype, int q_out_dtype, cudaStream_t stream);
+int launch_cache_read(const CacheReadArgs& args, int out_dtype, cudaStream_t stream);
+// Any storage type and head_dim, fp32 arithmetic.
+int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStream_t stream);
+// cudaFuncSetAttribute calls of the kernels, once per handle (not allowed to
+// fail later, inside a capture).
+int prepare_cache_attention_simt();
+
+}  // namespace awa
