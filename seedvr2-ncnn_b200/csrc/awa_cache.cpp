@@ -174,6 +174,8 @@ int create(const awa_cache_params* params, awa_cache** out, bool on_device)
         if (err == cudaSuccess)
             err = static_cast<cudaError_t>(awa::prepare_cache_attention_simt());
         if (err == cudaSuccess)
+            err = static_cast<cudaError_t>(awa::prepare_cache_attention_step());
+        if (err == cudaSuccess)
             cache->error_flag = awa::device_error_flag();
         if (err != cudaSuccess || !cache->error_flag)
         {
@@ -314,6 +316,15 @@ static int check_attention(const char* what, const awa_cache* cache, const awa_c
     return AWA_OK;
 }
 
+// No tile of max_rows rows sees more keys than this: the page table's reach,
+// and the prefix and the window.
+static int64_t most_seen(const awa::CacheAttnArgs& a, int max_rows)
+{
+    const int64_t reach = (int64_t)a.batch.table_width << a.mem.page_shift;
+    const int64_t window = a.sinks + (int64_t)a.window * a.frame_tokens + max_rows;
+    return a.window > 0 && window < reach ? window : reach;
+}
+
 size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int sinks,
                                            int window, int frame_tokens)
 {
@@ -370,9 +381,12 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
     a.window = window;
     a.frame_tokens = frame_tokens;
     a.error_flag = cache->error_flag;
-    return launch_status(
-        awa::launch_cache_attention_simt(a, batch->max_rows, static_cast<cudaStream_t>(stream)),
-        "awa_cache_attention launch");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool tensor = a.mem.storage != AWA_F32 && (a.mem.head_dim == 64 || a.mem.head_dim == 128);
+    const bool few = (int64_t)batch->max_rows * a.group <= 32;
+    const int err = tensor && few ? awa::launch_cache_attention_step(a, batch->max_rows, most_seen(a, batch->max_rows), s)
+                                  : awa::launch_cache_attention_simt(a, batch->max_rows, s);
+    return launch_status(err, "awa_cache_attention launch");
 }
 
 }  // extern "C"

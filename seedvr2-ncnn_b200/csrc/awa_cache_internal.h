@@ -84,8 +84,12 @@ int launch_cache_append(const CacheAppendArgs& args, int in_dtype, int q_out_dty
 int launch_cache_read(const CacheReadArgs& args, int out_dtype, cudaStream_t stream);
 // Any storage type and head_dim, fp32 arithmetic.
 int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStream_t stream);
+// bf16 and 4-bit caches with head_dim 64 or 128, for few rows per sequence;
+// most_keys: no row sees more.
+int launch_cache_attention_step(const CacheAttnArgs& args, int max_rows, int64_t most_keys, cudaStream_t stream);
 // cudaFuncSetAttribute calls of the kernels, once per handle (not allowed to
 // fail later, inside a capture).
 int prepare_cache_attention_simt();
+int prepare_cache_attention_step();
 
 }  // namespace awa

@@ -265,6 +265,23 @@ def test_a_page_shared_by_sequences_and_a_past_of_garbage(storage):
     assert ((got.double() - want).abs() <= tol).all()
 
 
+def test_4bit_groups_of_one_value_and_far_from_zero():
+    """Scale 0, a minimum many steps from 0, huge and tiny groups."""
+    c = Batch([2], [94], 16, 1, 128, "int4", seed=17)
+    x = torch.randn(96, 1, 128, device="cuda")
+    x[:20] = 3.0
+    x[20:30, :, :64] = 100 + 0.01 * x[20:30, :, :64]
+    x[30:40] *= 1e-30
+    x[40:50] = 0.0
+    x[50:60] = -1.001
+    packed, params = quantize(x)
+    page, slot = c.slots(0, torch.arange(96))
+    for t, p in ((c.k, c.params[0]), (c.v, c.params[1])):
+        t[page, :, slot], p[page, :, slot] = packed, params
+    for window in (0, 45, 60, 80):
+        attend(c, 4, 0, window, 1, torch.bfloat16, q_scale=0.3)
+
+
 # ---------------------------------------------------------------- together
 @pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
 def test_frames_through_append_and_attention(storage):
