@@ -176,6 +176,8 @@ int create(const awa_cache_params* params, awa_cache** out, bool on_device)
         if (err == cudaSuccess)
             err = static_cast<cudaError_t>(awa::prepare_cache_attention_step());
         if (err == cudaSuccess)
+            err = static_cast<cudaError_t>(awa::prepare_cache_attention_tile());
+        if (err == cudaSuccess)
             cache->error_flag = awa::device_error_flag();
         if (err != cudaSuccess || !cache->error_flag)
         {
@@ -384,8 +386,13 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool tensor = a.mem.storage != AWA_F32 && (a.mem.head_dim == 64 || a.mem.head_dim == 128);
     const bool few = (int64_t)batch->max_rows * a.group <= 32;
-    const int err = tensor && few ? awa::launch_cache_attention_step(a, batch->max_rows, most_seen(a, batch->max_rows), s)
-                                  : awa::launch_cache_attention_simt(a, batch->max_rows, s);
+    int err;
+    if (tensor && few)
+        err = awa::launch_cache_attention_step(a, batch->max_rows, most_seen(a, batch->max_rows), s);
+    else if (tensor && a.mem.storage == AWA_BF16 && a.group <= 128)
+        err = awa::launch_cache_attention_tile(a, s);
+    else
+        err = awa::launch_cache_attention_simt(a, batch->max_rows, s);
     return launch_status(err, "awa_cache_attention launch");
 }
 

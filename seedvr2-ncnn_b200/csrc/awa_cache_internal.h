@@ -87,9 +87,13 @@ int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStr
 // bf16 and 4-bit caches with head_dim 64 or 128, for few rows per sequence;
 // most_keys: no row sees more.
 int launch_cache_attention_step(const CacheAttnArgs& args, int max_rows, int64_t most_keys, cudaStream_t stream);
+// bf16 caches with head_dim 64 or 128 and at most 128 q heads per key/value
+// head, for many rows per sequence.
+int launch_cache_attention_tile(const CacheAttnArgs& args, cudaStream_t stream);
 // cudaFuncSetAttribute calls of the kernels, once per handle (not allowed to
 // fail later, inside a capture).
 int prepare_cache_attention_simt();
 int prepare_cache_attention_step();
+int prepare_cache_attention_tile();
 
 }  // namespace awa
