@@ -151,7 +151,10 @@ int awa_cache_read(const awa_cache* cache, const awa_cache_batch* batch, int out
  * statistics). 16-byte aligned rows. scale: > 0. sinks and window: 0 or more,
  * frame_tokens: 1 or more. Values in the cache that some row of the batch sees
  * have to be finite. workspace: awa_cache_attention_workspace_bytes() bytes,
- * 16-byte aligned (NULL if that is 0), used by this call until its work is done. */
+ * 16-byte aligned (NULL if that is 0), used by this call until its work is
+ * done: calls that may overlap, two captured graphs among them, need one each.
+ * It is 0 except for many rows over an AWA_INT4 cache, whose visible pages
+ * become bf16 in it (rounded once) ahead of the tensor cores. */
 size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int sinks,
                                            int window, int frame_tokens);
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,

@@ -327,15 +327,72 @@ static int64_t most_seen(const awa::CacheAttnArgs& a, int max_rows)
     return a.window > 0 && window < reach ? window : reach;
 }
 
+// The kernel that serves a call.
+enum Kernel
+{
+    kStep,        // few rows per head: bf16 and 4 bits
+    kTile,        // many rows: bf16
+    kUnpackTile,  // many rows of a 4-bit cache: its visible pages become bf16 first
+    kSimt
+};
+
+// Up to 32 (row, head) pairs per key/value head and sequence the step kernel
+// reads the keys once or twice at memory speed and fills its instructions; the
+// tile kernel always computes 128 of them.
+static Kernel kernel_of(const awa::CacheMemory& mem, int group, int max_rows)
+{
+    if (mem.storage == AWA_F32 || (mem.head_dim != 64 && mem.head_dim != 128))
+        return kSimt;
+    if ((int64_t)max_rows * group <= 32 || group > 128)
+        return kStep;
+    return mem.storage == AWA_INT4 ? kUnpackTile : kTile;
+}
+
+// Pages that the rows of a batch can see at most, all sequences together: the
+// whole table, or prefix, window and new rows with the pages they only touch.
+static int64_t most_pages(const awa::CacheMemory& mem, const awa::CacheBatch& batch, int sinks, int window,
+                          int frame_tokens)
+{
+    const int64_t all = (int64_t)batch.sequences * batch.table_width;
+    if (window == 0)
+        return all;
+    const auto pages = [&](int64_t tokens) { return (tokens + (1 << mem.page_shift) - 1) >> mem.page_shift; };
+    // a row's window and its frame, then rows - 1 more of them, ragged at both ends
+    const int64_t some = batch.sequences * (pages(sinks) + pages((int64_t)window * frame_tokens) + pages(frame_tokens) + 3) +
+                         pages(batch.rows);
+    return some < all ? some : all;
+}
+
+// The workspace of kUnpackTile: keys, values, page table, each on 256 bytes.
+struct Unpacked
+{
+    int64_t pages;
+    size_t page_bytes, pool_bytes, table_bytes;
+};
+
+static Unpacked unpacked_of(const awa::CacheMemory& mem, const awa::CacheBatch& batch, int sinks, int window,
+                            int frame_tokens)
+{
+    Unpacked u;
+    u.pages = most_pages(mem, batch, sinks, window, frame_tokens);
+    u.page_bytes = ((size_t)mem.heads * mem.head_dim * 2) << mem.page_shift;
+    u.pool_bytes = u.pages * u.page_bytes;
+    u.table_bytes = ((size_t)batch.sequences * batch.table_width * 4 + 255) / 256 * 256;
+    return u;
+}
+
 size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int sinks,
                                            int window, int frame_tokens)
 {
     awa::CacheBatch b;
     bool empty = false;
-    if (check_batch("awa_cache_attention_workspace_bytes", cache, batch, &b, &empty) ||
-        check_attention("awa_cache_attention_workspace_bytes", cache, batch, q_heads, sinks, window, frame_tokens))
+    static const char* const kWhat = "awa_cache_attention_workspace_bytes";
+    if (check_batch(kWhat, cache, batch, &b, &empty) ||
+        check_attention(kWhat, cache, batch, q_heads, sinks, window, frame_tokens) || empty ||
+        kernel_of(cache->mem, q_heads / cache->mem.heads, batch->max_rows) != kUnpackTile)
         return 0;
-    return 0;
+    const Unpacked u = unpacked_of(cache->mem, b, sinks, window, frame_tokens);
+    return 2 * u.pool_bytes + u.table_bytes;
 }
 
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,
@@ -384,15 +441,42 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
     a.frame_tokens = frame_tokens;
     a.error_flag = cache->error_flag;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool tensor = a.mem.storage != AWA_F32 && (a.mem.head_dim == 64 || a.mem.head_dim == 128);
-    const bool few = (int64_t)batch->max_rows * a.group <= 32;
-    int err;
-    if (tensor && few)
-        err = awa::launch_cache_attention_step(a, batch->max_rows, most_seen(a, batch->max_rows), s);
-    else if (tensor && a.mem.storage == AWA_BF16 && a.group <= 128)
+    int err = 0;
+    switch (kernel_of(a.mem, a.group, batch->max_rows))
+    {
+    case kStep: err = awa::launch_cache_attention_step(a, batch->max_rows, most_seen(a, batch->max_rows), s); break;
+    case kTile: err = awa::launch_cache_attention_tile(a, s); break;
+    case kSimt: err = awa::launch_cache_attention_simt(a, batch->max_rows, s); break;
+    case kUnpackTile:
+    {
+        const Unpacked u = unpacked_of(a.mem, a.batch, sinks, window, frame_tokens);
+        if (u.pages > 0x7fffffff)
+            return fail(AWA_ERR_INVALID, "awa_cache_attention: the batch reaches too many pages");
+        awa::CacheUnpackArgs unpack{};
+        unpack.mem = a.mem;
+        unpack.batch = a.batch;
+        unpack.sinks = sinks;
+        unpack.window = window;
+        unpack.frame_tokens = frame_tokens;
+        unpack.k_out = static_cast<char*>(workspace);
+        unpack.v_out = unpack.k_out + u.pool_bytes;
+        unpack.table = reinterpret_cast<int*>(unpack.v_out + u.pool_bytes);
+        unpack.error_flag = a.error_flag;
+        err = awa::launch_cache_unpack(unpack, (int)u.pages, s);
+        if (err)
+            break;
+        a.mem.storage = AWA_BF16;
+        a.mem.pages = (int)u.pages;
+        a.mem.k = unpack.k_out;
+        a.mem.v = unpack.v_out;
+        a.mem.page_stride = (int64_t)u.page_bytes;
+        a.mem.head_stride = (int64_t)u.page_bytes / a.mem.heads;
+        a.batch.page_table = unpack.table;
+        a.batch.table_stride = a.batch.table_width;
         err = awa::launch_cache_attention_tile(a, s);
-    else
-        err = awa::launch_cache_attention_simt(a, batch->max_rows, s);
+        break;
+    }
+    }
     return launch_status(err, "awa_cache_attention launch");
 }
 

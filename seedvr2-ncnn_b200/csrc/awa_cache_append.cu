@@ -20,6 +20,56 @@ using bf16 = __nv_bfloat16;
 constexpr int kThreads = 256;
 constexpr int kMaxTileRows = 8;
 
+// Page number `index` of all that the sequences of the batch see, counted
+// sequence by sequence. Called by one full warp; the same in all lanes.
+struct PageSlot
+{
+    int b;  // -1: none
+    int entry;
+};
+
+__device__ __forceinline__ PageSlot find_page(const CacheUnpackArgs& a, int index)
+{
+    const int lane = threadIdx.x & 31;
+    const int page = 1 << a.mem.page_shift;
+    int before = 0;
+    for (int base = 0; base < a.batch.sequences; base += 32)
+    {
+        const int b = base + lane;
+        KeyBlocks pages;
+        pages.prefix = pages.shift = pages.count = 0;
+        if (b < a.batch.sequences)
+        {
+            const int rows = batch_rows(a.batch, b);
+            const int past = max(0, __ldg(a.batch.past + b));
+            const int length = sequence_length(a.mem, a.batch, past, rows, nullptr);
+            if (rows > 0)
+                pages = key_blocks(row_span(min(past, length), length, a.sinks, a.window, a.frame_tokens),
+                                   row_span(min(past, length) + rows - 1, length, a.sinks, a.window, a.frame_tokens),
+                                   a.sinks, page);
+        }
+        int sum = pages.count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o)
+                sum += up;
+        }
+        const unsigned holds = __ballot_sync(0xffffffffu, index < before + sum);
+        if (holds)
+        {
+            const int src = __ffs(holds) - 1;
+            const int i = index - before - __shfl_sync(0xffffffffu, sum - pages.count, src);
+            const int prefix = __shfl_sync(0xffffffffu, pages.prefix, src);
+            const int shift = __shfl_sync(0xffffffffu, pages.shift, src);
+            return {base + src, i < prefix ? i : i + shift};
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return {-1, 0};
+}
+
 // 8 consecutive elements, in 16-byte pieces where the rows allow it.
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ void get8(const T* p, float (&v)[8])
@@ -285,6 +335,63 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheReadArgs a, i
     }
 }
 
+// One 4-bit page that some row of the batch sees -> its keys and values as
+// bf16, and its number in the workspace's page table. Blocks: x = the pages of
+// all sequences in order, y = heads.
+__global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs a)
+{
+    __shared__ int which_s[2];
+    const CacheMemory& mem = a.mem;
+    if (threadIdx.x < 32)
+    {
+        const PageSlot at = find_page(a, blockIdx.x);
+        if (threadIdx.x == 0)
+        {
+            which_s[0] = at.b;
+            which_s[1] = at.entry;
+        }
+    }
+    __syncthreads();
+    const int b = which_s[0], entry = which_s[1];
+    if (b < 0)
+        return;
+    const int page = __ldg(a.batch.page_table + b * a.batch.table_stride + entry);
+    const bool real = (unsigned)page < (unsigned)mem.pages;
+    if (threadIdx.x == 0 && blockIdx.y == 0)
+    {
+        if (!real)
+            cache_error(a.error_flag, AWA_CACHE_BAD_PAGE);
+        a.table[(int64_t)b * a.batch.table_width + entry] = blockIdx.x;
+    }
+    const int kv = blockIdx.y, groups = mem.head_dim / AWA_CACHE_GROUP, row_bytes = mem.head_dim / 2;
+    const int64_t page_bytes = (int64_t)row_bytes << mem.page_shift;  // of codes
+    const int64_t src = page * mem.page_stride + kv * mem.head_stride;
+    const int64_t par = page * mem.params_page_stride + kv * mem.params_head_stride;
+    const int64_t dst = ((int64_t)blockIdx.x * mem.heads + kv) * page_bytes * 4;
+    // 16 codes, of one group, a thread and turn
+    for (int i = threadIdx.x; i < 2 * (int)(page_bytes / 8); i += kThreads)
+    {
+        const bool is_k = i < (int)(page_bytes / 8);
+        const int at = (is_k ? i : i - (int)(page_bytes / 8)) * 8;
+        uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (real)
+        {
+            const uint2 codes = __ldg(reinterpret_cast<const uint2*>((is_k ? mem.k : mem.v) + src + at));
+            const int row = at / row_bytes, group = (at - row * row_bytes) / (AWA_CACHE_GROUP / 2);
+            const uint32_t params = __ldg(
+                reinterpret_cast<const uint32_t*>((is_k ? mem.k_params : mem.v_params) + par) + row * groups + group);
+            float v[8];
+            dequantize8(codes.x, params, v);
+            store8(reinterpret_cast<bf16*>(&out[0]), v);
+            dequantize8(codes.y, params, v);
+            store8(reinterpret_cast<bf16*>(&out[1]), v);
+        }
+        uint4* to = reinterpret_cast<uint4*>((is_k ? a.k_out : a.v_out) + dst + (int64_t)at * 4);
+        to[0] = out[0];
+        to[1] = out[1];
+    }
+}
+
 struct Shape
 {
     dim3 grid;
@@ -362,6 +469,13 @@ int launch_cache_read(const CacheReadArgs& a, int out_dtype, cudaStream_t stream
 {
     ProfileScope scope("awa_cache_read", stream);
     out_dtype == AWA_F32 ? run_read<float>(a, stream) : run_read<bf16>(a, stream);
+    return (int)cudaGetLastError();
+}
+
+int launch_cache_unpack(const CacheUnpackArgs& a, int pages, cudaStream_t stream)
+{
+    ProfileScope scope("awa_cache_unpack", stream);
+    cache_unpack_kernel<<<dim3((unsigned)pages, (unsigned)a.mem.heads), kThreads, 0, stream>>>(a);
     return (int)cudaGetLastError();
 }
 

@@ -11,8 +11,6 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
-#include <type_traits>
-
 namespace awa
 {
 namespace
@@ -35,32 +33,12 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, float acc)
     return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, acc))));
 }
 
-// 8 features of one cached row as floats.
-template <int ST>
-__device__ __forceinline__ void cached8(const char* row, const char* params, int f, float (&v)[8])
-{
-    if (ST == AWA_F32)
-        load8(reinterpret_cast<const float*>(row) + f, v);
-    else if (ST == AWA_BF16)
-        load8(reinterpret_cast<const bf16*>(row) + f, v);
-    else
-    {
-        const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(row + f / 2));
-        const uint32_t p = __ldg(reinterpret_cast<const uint32_t*>(params) + f / AWA_CACHE_GROUP);
-        const float scale = __uint_as_float(p << 16), minimum = __uint_as_float(p & 0xffff0000u);
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            v[i] = fmaf((float)((codes >> (4 * i)) & 15u), scale, minimum);
-    }
-}
-
-// A block (of a cluster of gridDim.x / tiles that share the keys) takes one
+// T: type of the cache, q and out. A block (of a cluster of gridDim.x / tiles that share the keys) takes one
 // tile of R * 16 query rows of one key/value head. Thread (ty, tx) of 16 x 16:
 // rows ty * R + i, keys tx + 16 j, output features 4 (tx + 16 j).
-template <int ST, int R>
+template <typename T, int R>
 __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAttnArgs a, int cluster_size)
 {
-    using T = typename std::conditional<ST == AWA_F32, float, bf16>::type;  // of q and out
     constexpr int kRows = 16 * R;
     extern __shared__ float4 shared4[];
     __shared__ QueryTile tile_s;
@@ -139,12 +117,9 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
                 if (page >= 0)
                 {
                     const int slot = key & ((1 << mem.page_shift) - 1);
-                    const int row_bytes = ST == AWA_INT4 ? d / 2 : d * (ST == AWA_F32 ? 4 : 2);
-                    const int64_t at = page * mem.page_stride + kv * mem.head_stride + (int64_t)slot * row_bytes;
-                    const int64_t par = page * mem.params_page_stride + kv * mem.params_head_stride +
-                                        (int64_t)slot * (d / AWA_CACHE_GROUP) * 4;
-                    cached8<ST>(mem.k + at, mem.k_params + par, f, k8);
-                    cached8<ST>(mem.v + at, mem.v_params + par, f, v8);
+                    const int64_t at = page * mem.page_stride + kv * mem.head_stride;
+                    load8(reinterpret_cast<const T*>(mem.k + at) + slot * d + f, k8);
+                    load8(reinterpret_cast<const T*>(mem.v + at) + slot * d + f, v8);
                 }
             }
             store8(sk + r * pitch + f, k8);
@@ -315,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
     cluster.sync();  // a block's shared memory stays until every peer has read it
 }
 
-template <int ST, int R>
+template <typename T, int R>
 int run(const CacheAttnArgs& a, cudaStream_t stream)
 {
     const int d = a.mem.head_dim;
@@ -341,15 +316,15 @@ int run(const CacheAttnArgs& a, cudaStream_t stream)
     attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&config, cache_attention_simt_kernel<ST, R>, a, cluster);
+    return (int)cudaLaunchKernelEx(&config, cache_attention_simt_kernel<T, R>, a, cluster);
 }
 
-template <int ST>
+template <typename T>
 int run(const CacheAttnArgs& a, int max_rows, cudaStream_t stream)
 {
     // 64 rows a tile use the FMA units best; up to 16 rows of a head group,
     // a tile of 16 does a quarter of the work
-    return (int64_t)max_rows * a.group <= 16 ? run<ST, 1>(a, stream) : run<ST, 4>(a, stream);
+    return (int64_t)max_rows * a.group <= 16 ? run<T, 1>(a, stream) : run<T, 4>(a, stream);
 }
 
 }  // namespace
@@ -357,12 +332,7 @@ int run(const CacheAttnArgs& a, int max_rows, cudaStream_t stream)
 int launch_cache_attention_simt(const CacheAttnArgs& a, int max_rows, cudaStream_t stream)
 {
     ProfileScope scope("awa_cache_attention_simt", stream);
-    switch (a.mem.storage)
-    {
-    case AWA_F32: return run<AWA_F32>(a, max_rows, stream);
-    case AWA_BF16: return run<AWA_BF16>(a, max_rows, stream);
-    default: return run<AWA_INT4>(a, max_rows, stream);
-    }
+    return a.mem.storage == AWA_F32 ? run<float>(a, max_rows, stream) : run<bf16>(a, max_rows, stream);
 }
 
 int prepare_cache_attention_simt()
@@ -371,10 +341,9 @@ int prepare_cache_attention_simt()
         return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     shared_floats(rows, kMaxHeadDim) * (int)sizeof(float));
     };
-    const void* kernels[3][2] = {
-        {(const void*)cache_attention_simt_kernel<AWA_F32, 1>, (const void*)cache_attention_simt_kernel<AWA_F32, 4>},
-        {(const void*)cache_attention_simt_kernel<AWA_BF16, 1>, (const void*)cache_attention_simt_kernel<AWA_BF16, 4>},
-        {(const void*)cache_attention_simt_kernel<AWA_INT4, 1>, (const void*)cache_attention_simt_kernel<AWA_INT4, 4>}};
+    const void* kernels[2][2] = {
+        {(const void*)cache_attention_simt_kernel<float, 1>, (const void*)cache_attention_simt_kernel<float, 4>},
+        {(const void*)cache_attention_simt_kernel<bf16, 1>, (const void*)cache_attention_simt_kernel<bf16, 4>}};
     for (auto& pair : kernels)
         for (int r = 0; r < 2; r++)
         {

@@ -118,6 +118,13 @@ __device__ __forceinline__ KeyBlocks key_blocks(RowSpan first, RowSpan last, int
     return k;
 }
 
+// Rows of sequence b; starts that reach outside the batch's rows get none there.
+__device__ __forceinline__ int batch_rows(const CacheBatch& batch, int b)
+{
+    const int start = __ldg(batch.row_starts + b), end = min(__ldg(batch.row_starts + b + 1), batch.rows);
+    return start < 0 ? 0 : max(0, end - start);
+}
+
 // A tile of query rows: m rows m0 .. m0 + count - 1 of sequence b, where row m
 // is head (m % group) of its group at row m / group of the sequence.
 struct QueryTile
@@ -146,9 +153,7 @@ __device__ __forceinline__ QueryTile find_tile(const CacheMemory& mem, const Cac
         if (b < batch.sequences)
         {
             start = __ldg(batch.row_starts + b);
-            // a batch whose starts reach outside its rows gets no rows from there
-            const int end = min(__ldg(batch.row_starts + b + 1), batch.rows);
-            rows = start < 0 ? 0 : max(0, end - start);
+            rows = batch_rows(batch, b);
         }
         const int tiles = (int)(((int64_t)rows * group + tile - 1) / tile);
         int sum = tiles;

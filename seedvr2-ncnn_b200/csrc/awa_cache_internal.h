@@ -66,6 +66,18 @@ struct CacheReadArgs
     int* error_flag;
 };
 
+// 4-bit pages that a batch sees -> dense bf16 pages [page][head][slot][head_dim]
+// and a page table [sequences][table_width] of theirs.
+struct CacheUnpackArgs
+{
+    CacheMemory mem;
+    CacheBatch batch;
+    int sinks, window, frame_tokens;
+    char *k_out, *v_out;
+    int* table;
+    int* error_flag;
+};
+
 struct CacheAttnArgs
 {
     CacheMemory mem;
@@ -82,7 +94,9 @@ struct CacheAttnArgs
 
 int launch_cache_append(const CacheAppendArgs& args, int in_dtype, int q_out_dtype, cudaStream_t stream);
 int launch_cache_read(const CacheReadArgs& args, int out_dtype, cudaStream_t stream);
-// Any storage type and head_dim, fp32 arithmetic.
+// pages: as many as the batch can see, at most.
+int launch_cache_unpack(const CacheUnpackArgs& args, int pages, cudaStream_t stream);
+// fp32 and bf16 caches of any head_dim, fp32 arithmetic.
 int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStream_t stream);
 // bf16 and 4-bit caches with head_dim 64 or 128, for few rows per sequence;
 // most_keys: no row sees more.
