@@ -153,8 +153,9 @@ int awa_cache_read(const awa_cache* cache, const awa_cache_batch* batch, int out
  * have to be finite. workspace: awa_cache_attention_workspace_bytes() bytes,
  * 16-byte aligned (NULL if that is 0), used by this call until its work is
  * done: calls that may overlap, two captured graphs among them, need one each.
- * It is 0 except for many rows over an AWA_INT4 cache, whose visible pages
- * become bf16 in it (rounded once) ahead of the tensor cores. */
+ * It holds the parts of rows that several blocks work on (few rows, long
+ * caches) and, for many rows over an AWA_INT4 cache, the visible pages as bf16
+ * (rounded once); other calls need none. */
 size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int sinks,
                                            int window, int frame_tokens);
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,

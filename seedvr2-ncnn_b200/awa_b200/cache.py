@@ -73,6 +73,13 @@ def _cache_library():
     return _lib
 
 
+def _current_raw_stream(index: int) -> int:
+    """cudaStream_t of the current stream of a device."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
+
+
 def rope_table(max_coord: int, pairs: int, base: float = 10000.0, device="cuda"):
     """[max_coord, pairs, 2] fp32 (cos, sin) of coord * base^(-i / pairs), the
     angles in float64 (exact where fp32 angles of far positions are not)."""
@@ -204,7 +211,11 @@ class KvCache:
     def _stream(self, batch: CacheBatch, stream):
         if batch.device != self.device:
             raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
-        return (_torch().cuda.current_stream(self.device) if stream is None else stream).cuda_stream
+        if stream is not None:
+            return stream.cuda_stream
+        # a step of one row takes the GPU a few microseconds; the Stream object
+        # that current_stream() builds would take the host two of its own
+        return _current_raw_stream(self.device.index) if self.device.index is not None else None
 
     def _empty(self, shape, dtype, stream):
         """New memory that belongs to the stream the call runs on: what the
@@ -214,6 +225,11 @@ class KvCache:
             return torch.empty(shape, dtype=dtype, device=self.device)
         with torch.cuda.stream(stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def _like(self, q, stream):
+        if stream is None and q.is_contiguous():
+            return _torch().empty_like(q)
+        return q.new_empty(q.shape) if stream is None else self._empty(q.shape, q.dtype, stream)
 
     def append(self, batch: CacheBatch, k, v, q=None, rope: Optional[CacheRope] = None, q_out=None, stream=None):
         """Writes the batch's k (rotated) and v rows into the cache; returns q
@@ -230,15 +246,18 @@ class KvCache:
             if rope.rows is not None and rope.rows != batch.rows:
                 raise ValueError(f"coords must have {batch.rows} rows")
         heads, qp, qs, op, os_, ot = 0, None, 0, None, 0, AWA_BF16
+        code = _dtype_code(k)
         if q is not None:
             heads, qp, qs = q.shape[1], q.data_ptr(), self._rows(batch, q, "q")
             if q_out is None:
-                q_out = self._empty(q.shape, q.dtype, stream)
+                q_out, os_, ot = self._like(q, stream), heads * self.head_dim, code
             elif q_out.shape != q.shape:
                 raise ValueError("q_out must have q's shape")
-            op, os_, ot = q_out.data_ptr(), self._rows(batch, q_out, "q_out"), _dtype_code(q_out)
-        rc = self._lib.awa_cache_append(self._handle, batch.ref, heads, _dtype_code(k), qp, qs, k.data_ptr(), ks,
-                                        v.data_ptr(), vs, None if rope is None else rope.ref, ot, op, os_, handle)
+            else:
+                os_, ot = self._rows(batch, q_out, "q_out"), _dtype_code(q_out)
+            op = q_out.data_ptr()
+        rc = self._lib.awa_cache_append(self._handle, batch.ref, heads, code, qp, qs, k.data_ptr(), ks, v.data_ptr(),
+                                        vs, None if rope is None else rope.ref, ot, op, os_, handle)
         if rc:
             _check(rc)
         return q_out if q is not None else None
@@ -263,28 +282,29 @@ class KvCache:
         """softmax(scale q K^T) V of every row over the cached rows it sees (scale
         1 / sqrt(head_dim) by default): [rows, q_heads, head_dim]. A workspace
         given must not be in use by another call; one made here is not shared."""
-        torch = _torch()
         handle = self._stream(batch, stream)
         if q.dtype != self._rows_dtype:
             raise TypeError(f"this cache takes {self._rows_dtype} rows")
-        qs = self._rows(batch, q, "q")
+        qs, heads = self._rows(batch, q, "q"), q.shape[1]
         if out is None:
-            out = self._empty(q.shape, q.dtype, stream)
+            out, os_ = self._like(q, stream), heads * self.head_dim
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out must have q's shape and dtype")
-        heads = q.shape[1]
-        need = self._lib.awa_cache_attention_workspace_bytes(self._handle, batch.ref, heads, sinks, window,
-                                                             frame_tokens)
-        space = None
+        else:
+            os_ = self._rows(batch, out, "out")
+        space, need = None, 0
+        if self.storage != AWA_F32:  # fp32 caches never need a workspace
+            need = self._lib.awa_cache_attention_workspace_bytes(self._handle, batch.ref, heads, sinks, window,
+                                                                 frame_tokens)
         if need:
             if workspace is None:
-                workspace = self._empty(need, torch.uint8, stream)
+                workspace = self._empty(need, _torch().uint8, stream)
             elif workspace.device != self.device:
                 raise ValueError(f"the workspace is on {workspace.device}, the cache on {self.device}")
             space, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         rc = self._lib.awa_cache_attention(self._handle, batch.ref, heads, self._type, q.data_ptr(), qs,
                                            self._scale if scale is None else scale, sinks, window, frame_tokens,
-                                           out.data_ptr(), self._rows(batch, out, "out"), space, need, handle)
+                                           out.data_ptr(), os_, space, need, handle)
         if rc:
             _check(rc)
         return out

@@ -320,11 +320,12 @@ static int check_attention(const char* what, const awa_cache* cache, const awa_c
 
 // No tile of max_rows rows sees more keys than this: the page table's reach,
 // and the prefix and the window.
-static int64_t most_seen(const awa::CacheAttnArgs& a, int max_rows)
+static int64_t most_seen(const awa::CacheMemory& mem, const awa_cache_batch& batch, int sinks, int window,
+                         int frame_tokens)
 {
-    const int64_t reach = (int64_t)a.batch.table_width << a.mem.page_shift;
-    const int64_t window = a.sinks + (int64_t)a.window * a.frame_tokens + max_rows;
-    return a.window > 0 && window < reach ? window : reach;
+    const int64_t reach = (int64_t)batch.table_width << mem.page_shift;
+    const int64_t seen = sinks + (int64_t)window * frame_tokens + batch.max_rows;
+    return window > 0 && seen < reach ? seen : reach;
 }
 
 // The kernel that serves a call.
@@ -388,8 +389,14 @@ size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cac
     bool empty = false;
     static const char* const kWhat = "awa_cache_attention_workspace_bytes";
     if (check_batch(kWhat, cache, batch, &b, &empty) ||
-        check_attention(kWhat, cache, batch, q_heads, sinks, window, frame_tokens) || empty ||
-        kernel_of(cache->mem, q_heads / cache->mem.heads, batch->max_rows) != kUnpackTile)
+        check_attention(kWhat, cache, batch, q_heads, sinks, window, frame_tokens) || empty)
+        return 0;
+    const int group = q_heads / cache->mem.heads;
+    const Kernel kernel = kernel_of(cache->mem, group, batch->max_rows);
+    if (kernel == kStep)
+        return awa::cache_attention_step_workspace(cache->mem, group, batch->max_rows,
+                                                   most_seen(cache->mem, *batch, sinks, window, frame_tokens));
+    if (kernel != kUnpackTile)
         return 0;
     const Unpacked u = unpacked_of(cache->mem, b, sinks, window, frame_tokens);
     return 2 * u.pool_bytes + u.table_bytes;
@@ -444,7 +451,10 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
     int err = 0;
     switch (kernel_of(a.mem, a.group, batch->max_rows))
     {
-    case kStep: err = awa::launch_cache_attention_step(a, batch->max_rows, most_seen(a, batch->max_rows), s); break;
+    case kStep:
+        err = awa::launch_cache_attention_step(a, batch->max_rows,
+                                               most_seen(a.mem, *batch, sinks, window, frame_tokens), workspace, s);
+        break;
     case kTile: err = awa::launch_cache_attention_tile(a, s); break;
     case kSimt: err = awa::launch_cache_attention_simt(a, batch->max_rows, s); break;
     case kUnpackTile:

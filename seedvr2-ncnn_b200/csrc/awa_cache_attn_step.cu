@@ -274,102 +274,93 @@ __device__ __forceinline__ void values(WarpState<ST, D, NQ>& w, const char* vdat
     }
 }
 
-// A cluster of `cluster_size` blocks takes one tile of 8 NQ query rows of one
-// key/value head; its warps take the stages of keys in turn.
-template <int ST, int D, int NQ>
-__global__ void __launch_bounds__(kThreads) cache_attention_step_kernel(CacheAttnArgs a, int cluster_size)
+// One piece of work of a block: a tile of query rows of one key/value head and
+// some of the key blocks that it sees.
+struct Piece
+{
+    QueryTile tile;
+    int kv;
+    KeyBlocks blocks;
+    RowSpan first, last;  // of the tile's rows
+    int begin, end;       // key blocks [begin, end) of `blocks`
+};
+
+__device__ __forceinline__ RowSpan tile_span(const CacheAttnArgs& a, const QueryTile& t, int m)
+{
+    return row_span(t.past + (t.m0 + m) / a.group, t.length, a.sinks, a.window, a.frame_tokens);
+}
+
+template <typename S>
+__device__ __forceinline__ int block_key(const Piece& p, int i)
+{
+    return (i < p.blocks.prefix ? i : i + p.blocks.shift) * S::kKeys;
+}
+
+// Issues the copies of key block i of the piece into stage `slot` of the warp's ring.
+template <int ST, int D>
+__device__ __forceinline__ void issue_block(const CacheAttnArgs& a, const Piece& p, int i, char* ring, int slot)
 {
     using S = Step<ST, D>;
-    constexpr int kRows = 8 * NQ;
-    extern __shared__ __align__(128) char shared[];
-    __shared__ QueryTile tile_s;
-    __shared__ float2 ml_s[kWarps + 1][kRows];  // maximum and sum: of each warp, then of the block
     const CacheMemory& mem = a.mem;
-    const int rank = blockIdx.x % cluster_size;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    if (warp == 0)
-    {
-        const QueryTile found =
-            find_tile(mem, a.batch, a.group, kRows, blockIdx.x / cluster_size, rank == 0 ? a.error_flag : nullptr);
-        if (lane == 0)
-            tile_s = found;
-    }
-    __syncthreads();
-    const QueryTile tile = tile_s;
-    if (tile.b < 0)
-        return;  // the whole cluster
-    const int kv = blockIdx.y;
-
-    const auto span_of = [&](int m) {
-        return row_span(tile.past + (tile.m0 + m) / a.group, tile.length, a.sinks, a.window, a.frame_tokens);
-    };
-    const RowSpan first = span_of(0), last = span_of(tile.count - 1);
-    const KeyBlocks blocks = key_blocks(first, last, a.sinks, S::kKeys);
-    const int parts = cluster_size * kWarps;
-    char* ring = shared + warp * S::kWarpBytes;
-    float2* scales = reinterpret_cast<float2*>(ring + kStages * S::kStageBytes);
-    const char* kbase = mem.k + kv * mem.head_stride;
-    const char* vbase = mem.v + kv * mem.head_stride;
-    const int* table = a.batch.page_table + tile.b * a.batch.table_stride;
+    const int lane = threadIdx.x & 31;
+    const int* table = a.batch.page_table + p.tile.b * a.batch.table_stride;
     const int page_mask = (1 << mem.page_shift) - 1;
-
-    // Issues the copies of stage n of this warp (n counts from 0) into the ring.
-    const auto issue = [&](int n) {
-        const int i = rank * kWarps + warp + n * parts;
-        if (i < blocks.count)
+    const int key0 = block_key<S>(p, i);
+    const uint32_t dst = shared_address(ring) + slot * S::kStageBytes;
+    // only what some row sees is read: pages outside may be gone
+    const auto seen = [&](int key) { return key < p.last.hi && (key >= p.first.lo || key < a.sinks); };
+    const bool all = key0 + S::kKeys <= p.last.hi && (key0 >= p.first.lo || key0 + S::kKeys <= a.sinks);
+    constexpr int kPieces = S::kRowBytes / 16;  // a power of two: 2, 4, 8 or 16
+    const char* kbase = mem.k + p.kv * mem.head_stride;
+    const char* vbase = mem.v + p.kv * mem.head_stride;
+#pragma unroll
+    for (int j = 0; j < S::kKeys * kPieces / 32; j++)
+    {
+        const int r = (j * 32 + lane) / kPieces, c = (j * 32 + lane) % kPieces;
+        const int key = key0 + r;
+        bool real = all || seen(key);
+        int page = real ? __ldg(table + (key >> mem.page_shift)) : 0;
+        if ((unsigned)page >= (unsigned)mem.pages)
         {
-            const int key0 = (i < blocks.prefix ? i : i + blocks.shift) * S::kKeys;
-            const uint32_t dst = shared_address(ring) + (n % kStages) * S::kStageBytes;
-            const bool all = key0 + S::kKeys <= last.hi && (key0 >= first.lo || key0 + S::kKeys <= a.sinks);
-            constexpr int kPieces = S::kRowBytes / 16;  // a power of two: 2, 4, 8 or 16
-#pragma unroll
-            for (int j = 0; j < S::kKeys * kPieces / 32; j++)
-            {
-                const int r = (j * 32 + lane) / kPieces, c = (j * 32 + lane) % kPieces;
-                const int key = key0 + r;
-                // only what some row sees is read: pages outside may be gone
-                bool real = all || (key < last.hi && (key >= first.lo || key < a.sinks));
-                int page = real ? __ldg(table + (key >> mem.page_shift)) : 0;
-                if ((unsigned)page >= (unsigned)mem.pages)
-                {
-                    cache_error(a.error_flag, AWA_CACHE_BAD_PAGE);
-                    page = 0;
-                    real = false;
-                }
-                const int64_t at = page * mem.page_stride + (int64_t)(key & page_mask) * S::kRowBytes + 16 * c;
-                const int to = piece_offset<ST, D>(r, c);
-                copy_async<16>(dst + to, kbase + at, real);
-                copy_async<16>(dst + S::kKeys * S::kRowBytes + to, vbase + at, real);
-            }
-            if (S::kFour)
-            {
-                const int key = key0 + lane;
-                bool real = all || (key < last.hi && (key >= first.lo || key < a.sinks));
-                int page = real ? __ldg(table + (key >> mem.page_shift)) : 0;
-                real = real && (unsigned)page < (unsigned)mem.pages;
-                page = real ? page : 0;
-                const int64_t at = page * mem.params_page_stride + kv * mem.params_head_stride +
-                                   (int64_t)(key & page_mask) * S::kParamBytes;
-                const uint32_t to = dst + 2 * S::kKeys * S::kRowBytes + lane * S::kParamBytes;
-                copy_async<S::kFour ? S::kParamBytes : 4>(to, mem.k_params + at, real);
-                copy_async<S::kFour ? S::kParamBytes : 4>(to + S::kKeys * S::kParamBytes, mem.v_params + at, real);
-            }
+            cache_error(a.error_flag, AWA_CACHE_BAD_PAGE);
+            page = 0;
+            real = false;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int n = 0; n < kStages - 1; n++)
-        issue(n);
+        const int64_t at = page * mem.page_stride + (int64_t)(key & page_mask) * S::kRowBytes + 16 * c;
+        const int to = piece_offset<ST, D>(r, c);
+        copy_async<16>(dst + to, kbase + at, real);
+        copy_async<16>(dst + S::kKeys * S::kRowBytes + to, vbase + at, real);
+    }
+    if (S::kFour)
+    {
+        const int key = key0 + lane;
+        bool real = all || seen(key);
+        int page = real ? __ldg(table + (key >> mem.page_shift)) : 0;
+        real = real && (unsigned)page < (unsigned)mem.pages;
+        page = real ? page : 0;
+        const int64_t at = page * mem.params_page_stride + p.kv * mem.params_head_stride +
+                           (int64_t)(key & page_mask) * S::kParamBytes;
+        const uint32_t to = dst + 2 * S::kKeys * S::kRowBytes + lane * S::kParamBytes;
+        copy_async<S::kFour ? S::kParamBytes : 4>(to, mem.k_params + at, real);
+        copy_async<S::kFour ? S::kParamBytes : 4>(to + S::kKeys * S::kParamBytes, mem.v_params + at, real);
+    }
+}
 
-    WarpState<ST, D, NQ> w;
+// The tile's queries as operands, and an empty state.
+template <int ST, int D, int NQ>
+__device__ __forceinline__ void start(const CacheAttnArgs& a, const Piece& p, WarpState<ST, D, NQ>& w)
+{
+    using S = Step<ST, D>;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const bf16* q = static_cast<const bf16*>(a.q);
 #pragma unroll
     for (int n = 0; n < NQ; n++)
     {
         // column g of tile n
-        const int m = tile.m0 + n * 8 + g;
-        const bool mine = n * 8 + g < tile.count;
-        const bf16* row = q + (int64_t)(tile.row0 + m / a.group) * a.q_stride + (int64_t)(kv * a.group + m % a.group) * D;
+        const int m = p.tile.m0 + n * 8 + g;
+        const bool mine = n * 8 + g < p.tile.count;
+        const bf16* row =
+            q + (int64_t)(p.tile.row0 + m / a.group) * a.q_stride + (int64_t)(p.kv * a.group + m % a.group) * D;
         float part[S::kGroups] = {};
         if (ST == AWA_INT4)
 #pragma unroll
@@ -420,122 +411,195 @@ __global__ void __launch_bounds__(kThreads) cache_attention_step_kernel(CacheAtt
         {
             w.top[n][c] = -INFINITY;
             w.sum[n][c] = 0.f;
-            w.span[n][c] = span_of(min(n * 8 + 2 * t + c, tile.count - 1));
+            w.span[n][c] = tile_span(a, p.tile, min(n * 8 + 2 * t + c, p.tile.count - 1));
         }
     }
-    const float to_log2 = a.scale * 1.44269504088896341f;
+}
 
+// One key block, arrived in the ring.
+template <int ST, int D, int NQ>
+__device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, WarpState<ST, D, NQ>& w, int key0,
+                                        const char* kdata, float2* scales)
+{
+    using S = Step<ST, D>;
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    const float to_log2 = a.scale * 1.44269504088896341f;
+    const char* vdata = kdata + S::kKeys * S::kRowBytes;
+    if (S::kFour)
+    {
+        // a lane works out (scale, z - 128) of its key. A scale of 0 or next
+        // to it (then the value is the minimum) is raised to where z and
+        // scale z stay finite: that moves the value by 15 * 2^-100 of it
+        const uint32_t* par = reinterpret_cast<const uint32_t*>(vdata + S::kKeys * S::kRowBytes);
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int gr = 0; gr < S::kGroups; gr++)
+            {
+                const uint32_t word = par[(x * S::kKeys + lane) * S::kGroups + gr];
+                const float low = __uint_as_float(word & 0xffff0000u);
+                const float scale = fmaxf(__uint_as_float(word << 16), 0x1p-100f * fmaxf(1.f, fabsf(low)));
+                scales[(x * S::kKeys + lane) * S::kGroups + gr] = make_float2(scale, __fdividef(low, scale) - 128.f);
+            }
+        __syncwarp();
+    }
+    constexpr int kBlocks = S::kKeys / 16;
+    float s[kBlocks][NQ][4];
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+        scores<ST, D, NQ>(w, kdata, scales, b, s[b]);
+    // rows of the tile see all of these keys: nothing to mask
+    const bool all = key0 + S::kKeys <= p.first.hi && (key0 >= p.last.lo || key0 + S::kKeys <= a.sinks);
+    if (!all)
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int x = 0; x < NQ; x++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                {
+                    const int key = key0 + b * 16 + key_of_row<ST>(g) + (c < 2 ? 0 : 8);
+                    const RowSpan& span = w.span[x][c & 1];
+                    if (!(key < span.hi && (key >= span.lo || key < a.sinks)))
+                        s[b][x][c] = -INFINITY;
+                }
+    float base[NQ][2];
+    bool grew = false;
+#pragma unroll
+    for (int x = 0; x < NQ; x++)
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+        {
+            float top = fmaxf(s[0][x][c], s[0][x][c + 2]);
+#pragma unroll
+            for (int b = 1; b < kBlocks; b++)
+                top = fmaxf(top, fmaxf(s[b][x][c], s[b][x][c + 2]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            base[x][c] = fmaxf(top, w.top[x][c]);
+            grew |= top > w.top[x][c];
+        }
+    if (__any_sync(0xffffffffu, grew))
+#pragma unroll
+        for (int x = 0; x < NQ; x++)
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+            {
+                const float old = w.top[x][c] == base[x][c] ? 1.f : fast_exp2((w.top[x][c] - base[x][c]) * to_log2);
+                w.top[x][c] = base[x][c];
+                w.sum[x][c] *= old;
+#pragma unroll
+                for (int gr = 0; gr < S::kGroups; gr++)
+                    w.off[x][gr][c] *= old;
+#pragma unroll
+                for (int j = 0; j < D / 16; j++)
+                {
+                    w.o[x][j][c] *= old;
+                    w.o[x][j][c + 2] *= old;
+                }
+            }
+#pragma unroll
+    for (int x = 0; x < NQ; x++)
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+        {
+            // nothing seen yet: all exponentials are 0
+            const float from = base[x][c] == -INFINITY ? 0.f : base[x][c] * to_log2;
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+            {
+                s[b][x][c] = fast_exp2(fmaf(s[b][x][c], to_log2, -from));
+                s[b][x][c + 2] = fast_exp2(fmaf(s[b][x][c + 2], to_log2, -from));
+                w.sum[x][c] += s[b][x][c] + s[b][x][c + 2];
+            }
+        }
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+        values<ST, D, NQ>(w, vdata, scales + S::kKeys * S::kGroups, b, s[b]);
+}
+
+// The warp's share of the piece: key blocks begin + turn, + turns, ...
+template <int ST, int D, int NQ>
+__device__ __forceinline__ void work(const CacheAttnArgs& a, const Piece& p, WarpState<ST, D, NQ>& w, char* ring,
+                                     int turn, int turns)
+{
+    using S = Step<ST, D>;
+    float2* scales = reinterpret_cast<float2*>(ring + kStages * S::kStageBytes);
+    const auto issue = [&](int n) {
+        const int i = p.begin + turn + n * turns;
+        if (i < p.end)
+            issue_block<ST, D>(a, p, i, ring, n % kStages);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int n = 0; n < kStages - 1; n++)
+        issue(n);
+    start<ST, D, NQ>(a, p, w);
     for (int n = 0;; n++)
     {
-        const int i = rank * kWarps + warp + n * parts;
-        if (i >= blocks.count)
+        const int i = p.begin + turn + n * turns;
+        if (i >= p.end)
             break;
         issue(n + kStages - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
-        const char* kdata = ring + (n % kStages) * S::kStageBytes;
-        const char* vdata = kdata + S::kKeys * S::kRowBytes;
-        const int key0 = (i < blocks.prefix ? i : i + blocks.shift) * S::kKeys;
-        if (S::kFour)
-        {
-            // a lane works out (scale, z - 128) of its key. A scale of 0 or next
-            // to it (then the value is the minimum) is raised to where z and
-            // scale z stay finite: that moves the value by 15 * 2^-100 of it
-            const uint32_t* par = reinterpret_cast<const uint32_t*>(vdata + S::kKeys * S::kRowBytes);
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int gr = 0; gr < S::kGroups; gr++)
-                {
-                    const uint32_t word = par[(x * S::kKeys + lane) * S::kGroups + gr];
-                    const float low = __uint_as_float(word & 0xffff0000u);
-                    const float scale = fmaxf(__uint_as_float(word << 16), 0x1p-100f * fmaxf(1.f, fabsf(low)));
-                    scales[(x * S::kKeys + lane) * S::kGroups + gr] =
-                        make_float2(scale, __fdividef(low, scale) - 128.f);
-                }
-            __syncwarp();
-        }
-        constexpr int kBlocks = S::kKeys / 16;
-        float s[kBlocks][NQ][4];
-#pragma unroll
-        for (int b = 0; b < kBlocks; b++)
-            scores<ST, D, NQ>(w, kdata, scales, b, s[b]);
-        // rows of the tile see all of these keys: nothing to mask
-        const bool all = (key0 >= last.lo && key0 + S::kKeys <= first.hi) ||
-                         (key0 + S::kKeys <= a.sinks && key0 + S::kKeys <= first.hi);
-        if (!all)
-#pragma unroll
-            for (int b = 0; b < kBlocks; b++)
-#pragma unroll
-                for (int x = 0; x < NQ; x++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                    {
-                        const int key = key0 + b * 16 + key_of_row<ST>(g) + (c < 2 ? 0 : 8);
-                        const RowSpan& span = w.span[x][c & 1];
-                        if (!(key < span.hi && (key >= span.lo || key < a.sinks)))
-                            s[b][x][c] = -INFINITY;
-                    }
-        float base[NQ][2];
-        bool grew = false;
-#pragma unroll
-        for (int x = 0; x < NQ; x++)
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-            {
-                float top = fmaxf(s[0][x][c], s[0][x][c + 2]);
-#pragma unroll
-                for (int b = 1; b < kBlocks; b++)
-                    top = fmaxf(top, fmaxf(s[b][x][c], s[b][x][c + 2]));
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1)
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                base[x][c] = fmaxf(top, w.top[x][c]);
-                grew |= top > w.top[x][c];
-            }
-        if (__any_sync(0xffffffffu, grew))
-#pragma unroll
-            for (int x = 0; x < NQ; x++)
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-                {
-                    const float old = w.top[x][c] == base[x][c] ? 1.f : fast_exp2((w.top[x][c] - base[x][c]) * to_log2);
-                    w.top[x][c] = base[x][c];
-                    w.sum[x][c] *= old;
-#pragma unroll
-                    for (int gr = 0; gr < S::kGroups; gr++)
-                        w.off[x][gr][c] *= old;
-#pragma unroll
-                    for (int j = 0; j < D / 16; j++)
-                    {
-                        w.o[x][j][c] *= old;
-                        w.o[x][j][c + 2] *= old;
-                    }
-                }
-#pragma unroll
-        for (int x = 0; x < NQ; x++)
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-            {
-                // nothing seen yet: all exponentials are 0
-                const float from = base[x][c] == -INFINITY ? 0.f : base[x][c] * to_log2;
-#pragma unroll
-                for (int b = 0; b < kBlocks; b++)
-                {
-                    s[b][x][c] = fast_exp2(fmaf(s[b][x][c], to_log2, -from));
-                    s[b][x][c + 2] = fast_exp2(fmaf(s[b][x][c + 2], to_log2, -from));
-                    w.sum[x][c] += s[b][x][c] + s[b][x][c + 2];
-                }
-            }
-#pragma unroll
-        for (int b = 0; b < kBlocks; b++)
-            values<ST, D, NQ>(w, vdata, scales + S::kKeys * S::kGroups, b, s[b]);
+        consume<ST, D, NQ>(a, p, w, block_key<S>(p, i), ring + (n % kStages) * S::kStageBytes, scales);
         __syncwarp();  // the stage is free for the copies of the next round
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();  // the rings become the partial results [warp][row][feature]
+}
 
-    float* parts_s = reinterpret_cast<float*>(shared);
+// Joins the parts of `parts` holders of (maximum, sum) and unnormalised
+// outputs, in their order: ml(i) and o(i) of this thread's row and two features.
+struct Joined
+{
+    float top, total;
+    float2 o;
+};
+
+template <typename Ml, typename O>
+__device__ __forceinline__ Joined join(int parts, float to_log2, Ml ml, O o)
+{
+    Joined j;
+    j.top = -INFINITY;
+    for (int i = 0; i < parts; i++)
+        j.top = fmaxf(j.top, ml(i).x);
+    const float from = j.top == -INFINITY ? 0.f : j.top;
+    j.total = 0.f;
+    j.o = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < parts; i++)
+    {
+        const float2 x = ml(i), y = o(i);
+        const float f = fast_exp2((x.x - from) * to_log2);
+        j.total = fmaf(x.y, f, j.total);
+        j.o.x = fmaf(y.x, f, j.o.x);
+        j.o.y = fmaf(y.y, f, j.o.y);
+    }
+    return j;
+}
+
+template <int D>
+__device__ __forceinline__ void store_out(const CacheAttnArgs& a, const QueryTile& t, int kv, int r, int f,
+                                          const Joined& j)
+{
+    // a row that sees nothing gets zeros
+    const float inv = j.total == 0.f ? 0.f : 1.f / j.total;
+    const int m = t.m0 + r;
+    *reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) + (int64_t)(t.row0 + m / a.group) * a.out_stride +
+                                 (int64_t)(kv * a.group + m % a.group) * D + f) =
+        pack_bf16x2(j.o.x * inv, j.o.y * inv);
+}
+
+// Warp results -> shared memory [warp][row][feature] and ml [warp][row], the
+// rings' place; a block barrier before and after.
+template <int ST, int D, int NQ>
+__device__ __forceinline__ void publish(const WarpState<ST, D, NQ>& w, float* parts, float2 (*ml)[8 * NQ])
+{
+    using S = Step<ST, D>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    __syncthreads();
 #pragma unroll
     for (int x = 0; x < NQ; x++)
 #pragma unroll
@@ -557,103 +621,380 @@ __global__ void __launch_bounds__(kThreads) cache_attention_step_kernel(CacheAtt
                         off[gr] += __shfl_xor_sync(0xffffffffu, off[gr], o);
             }
             if (g == 0)
-                ml_s[warp][r] = make_float2(w.top[x][c], sum);
+                ml[warp][r] = make_float2(w.top[x][c], sum);
 #pragma unroll
             for (int j = 0; j < D / 16; j++)
 #pragma unroll
                 for (int h = 0; h < 2; h++)
                 {
                     const int f = S::kFour ? 64 * (j / 4) + 8 * g + 4 * h + j % 4 : 16 * j + 8 * h + g;
-                    parts_s[(warp * kRows + r) * S::kPitch + f] = w.o[x][j][c + 2 * h] + (S::kFour ? off[j / 4] : 0.f);
+                    parts[(warp * 8 * NQ + r) * S::kPitch + f] = w.o[x][j][c + 2 * h] + (S::kFour ? off[j / 4] : 0.f);
                 }
         }
     __syncthreads();
+}
 
-    // The block's warps, then the cluster's blocks, joined in a fixed order.
-    bf16* out = static_cast<bf16*>(a.out);
-    const auto store = [&](int r, int f, float2 v, float total) {
-        const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-        const int m = tile.m0 + r;
-        *reinterpret_cast<uint32_t*>(out + (int64_t)(tile.row0 + m / a.group) * a.out_stride +
-                                     (int64_t)(kv * a.group + m % a.group) * D + f) =
-            pack_bf16x2(v.x * inv, v.y * inv);
-    };
+// Short caches: a cluster of `cluster_size` blocks takes one tile of 8 NQ query
+// rows of one key/value head, its warps the key blocks in turn, and the blocks
+// join their parts in each other's shared memory: one launch, no workspace.
+template <int ST, int D, int NQ>
+__global__ void __launch_bounds__(kThreads) cache_attention_step_kernel(CacheAttnArgs a, int cluster_size)
+{
+    using S = Step<ST, D>;
+    constexpr int kRows = 8 * NQ;
+    extern __shared__ __align__(128) char shared[];
+    __shared__ QueryTile tile_s;
+    __shared__ float2 ml_s[kWarps + 1][kRows];  // maximum and sum: of each warp, then of the block
+    const int rank = blockIdx.x % cluster_size;
+    const int warp = threadIdx.x >> 5;
+    if (warp == 0)
+    {
+        const QueryTile found =
+            find_tile(a.mem, a.batch, a.group, kRows, blockIdx.x / cluster_size, rank == 0 ? a.error_flag : nullptr);
+        if (threadIdx.x == 0)
+            tile_s = found;
+    }
+    __syncthreads();
+    Piece p;
+    p.tile = tile_s;
+    if (p.tile.b < 0)
+        return;  // the whole cluster
+    p.kv = blockIdx.y;
+    p.first = tile_span(a, p.tile, 0);
+    p.last = tile_span(a, p.tile, p.tile.count - 1);
+    p.blocks = key_blocks(p.first, p.last, a.sinks, S::kKeys);
+    p.begin = 0;
+    p.end = p.blocks.count;
+    WarpState<ST, D, NQ> w;
+    work<ST, D, NQ>(a, p, w, shared + warp * S::kWarpBytes, rank * kWarps + warp, cluster_size * kWarps);
+    float* parts_s = reinterpret_cast<float*>(shared);
+    publish<ST, D, NQ>(w, parts_s, ml_s);
+
+    const float to_log2 = a.scale * 1.44269504088896341f;
     float* block_s = parts_s + kWarps * kRows * S::kPitch;
-    for (int e = threadIdx.x; e < tile.count * (D / 2); e += kThreads)
+    for (int e = threadIdx.x; e < p.tile.count * (D / 2); e += kThreads)
     {
         const int r = e / (D / 2), f = 2 * (e % (D / 2));
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kWarps; i++)
-            top = fmaxf(top, ml_s[i][r].x);
-        const float from = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
-        float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < kWarps; i++)
-        {
-            const float2 ml = ml_s[i][r];
-            const float x = fast_exp2((ml.x - from) * to_log2);
-            const float2 y = *reinterpret_cast<const float2*>(parts_s + (i * kRows + r) * S::kPitch + f);
-            total = fmaf(ml.y, x, total);
-            v.x = fmaf(y.x, x, v.x);
-            v.y = fmaf(y.y, x, v.y);
-        }
+        const Joined j = join(
+            kWarps, to_log2, [&](int i) { return ml_s[i][r]; },
+            [&](int i) { return *reinterpret_cast<const float2*>(parts_s + (i * kRows + r) * S::kPitch + f); });
         if (cluster_size == 1)
-            store(r, f, v, total);
+            store_out<D>(a, p.tile, p.kv, r, f, j);
         else
         {
-            *reinterpret_cast<float2*>(block_s + r * S::kPitch + f) = v;
+            *reinterpret_cast<float2*>(block_s + r * S::kPitch + f) = j.o;
             if (f == 0)
-                ml_s[kWarps][r] = make_float2(top, total);
+                ml_s[kWarps][r] = make_float2(j.top, j.total);
         }
     }
     if (cluster_size == 1)
         return;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    for (int e = rank * kThreads + threadIdx.x; e < tile.count * (D / 2); e += cluster_size * kThreads)
+    for (int e = rank * kThreads + threadIdx.x; e < p.tile.count * (D / 2); e += cluster_size * kThreads)
     {
         const int r = e / (D / 2), f = 2 * (e % (D / 2));
-        float top = -INFINITY;
-        for (int i = 0; i < cluster_size; i++)
-            top = fmaxf(top, cluster.map_shared_rank(&ml_s[kWarps][r], i)->x);
-        const float from = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
-        float2 v = make_float2(0.f, 0.f);
-        for (int i = 0; i < cluster_size; i++)
-        {
-            const float2 ml = *cluster.map_shared_rank(&ml_s[kWarps][r], i);
-            const float x = fast_exp2((ml.x - from) * to_log2);
-            const float2 y = *reinterpret_cast<const float2*>(cluster.map_shared_rank(block_s, i) + r * S::kPitch + f);
-            total = fmaf(ml.y, x, total);
-            v.x = fmaf(y.x, x, v.x);
-            v.y = fmaf(y.y, x, v.y);
-        }
-        store(r, f, v, total);
+        const Joined j = join(
+            cluster_size, to_log2, [&](int i) { return *cluster.map_shared_rank(&ml_s[kWarps][r], i); },
+            [&](int i) {
+                return *reinterpret_cast<const float2*>(cluster.map_shared_rank(block_s, i) + r * S::kPitch + f);
+            });
+        store_out<D>(a, p.tile, p.kv, r, f, j);
     }
     cluster.sync();  // a block's shared memory stays until every peer has read it
 }
 
+// ---------------------------------------------------------------- long caches
+// The work of a batch in rounds of kWarps key blocks, counted sequence by
+// sequence, head by head, tile by tile. Every tile of a sequence counts the
+// rounds of all of its rows, so that a sequence is (tiles * heads) equal parts.
+struct Rounds
+{
+    int tiles;   // of the sequence
+    int per;     // rounds of one tile and head
+};
+
+template <typename S>
+__device__ __forceinline__ Rounds sequence_rounds(const CacheAttnArgs& a, int b, int tile)
+{
+    Rounds r = {0, 0};
+    const int rows = b < a.batch.sequences ? batch_rows(a.batch, b) : 0;
+    if (rows > 0)
+    {
+        const int past = max(0, __ldg(a.batch.past + b));
+        const int length = sequence_length(a.mem, a.batch, past, rows, nullptr);
+        const int p0 = min(past, length);
+        const KeyBlocks k = key_blocks(row_span(p0, length, a.sinks, a.window, a.frame_tokens),
+                                       row_span(p0 + rows - 1, length, a.sinks, a.window, a.frame_tokens), a.sinks,
+                                       S::kKeys);
+        r.tiles = (int)(((int64_t)rows * a.group + tile - 1) / tile);
+        r.per = max(1, (k.count + kWarps - 1) / kWarps);
+    }
+    return r;
+}
+
+// Where a round lies: sequence b, whose first round is `before`. Warp-collective.
+struct Place
+{
+    int b;  // -1: past the end
+    Rounds r;
+    int64_t before;
+};
+
+template <typename S>
+__device__ __forceinline__ Place find_round(const CacheAttnArgs& a, int tile, int64_t round, int64_t* total)
+{
+    const int lane = threadIdx.x & 31;
+    Place place;
+    place.b = -1;
+    int64_t before = 0;
+    for (int base = 0; base < a.batch.sequences; base += 32)
+    {
+        const Rounds r = sequence_rounds<S>(a, base + lane, tile);
+        const int64_t mine = (int64_t)r.tiles * a.mem.heads * r.per;
+        int64_t sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o)
+                sum += up;
+        }
+        const unsigned holds = __ballot_sync(0xffffffffu, round < before + sum);
+        if (!total && holds)
+        {
+            const int src = __ffs(holds) - 1;
+            place.b = base + src;
+            place.r.tiles = __shfl_sync(0xffffffffu, r.tiles, src);
+            place.r.per = __shfl_sync(0xffffffffu, r.per, src);
+            place.before = before + __shfl_sync(0xffffffffu, sum - mine, src);
+            return place;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (total)
+        *total = before;
+    return place;
+}
+
+// The blocks among which `total` rounds are dealt: each gets 4 rounds or more.
+__device__ __forceinline__ int dealt(int64_t total, int blocks)
+{
+    return (int)max((int64_t)1, min((int64_t)blocks, total / 4));
+}
+
+// Block c of n has the rounds [first_round(c), first_round(c + 1)).
+__device__ __forceinline__ int64_t first_round(int64_t total, int n, int c)
+{
+    return total * c / n;
+}
+
+// Tile number `tile` of sequence b, tiles of `size` (row, head) pairs.
+__device__ __forceinline__ QueryTile tile_of(const CacheAttnArgs& a, int b, int tile, int size, int* flag)
+{
+    QueryTile t;
+    t.b = b;
+    t.row0 = __ldg(a.batch.row_starts + b);
+    const int rows = batch_rows(a.batch, b);
+    t.m0 = tile * size;
+    t.count = min(size, rows * a.group - t.m0);
+    t.past = max(0, __ldg(a.batch.past + b));
+    t.length = sequence_length(a.mem, a.batch, t.past, rows, flag);
+    t.past = min(t.past, t.length);
+    return t;
+}
+
+// Long caches: every block takes an equal share of the batch's rounds, however
+// the sequences differ in length. A tile that one block has whole is finished
+// there; the parts of the others go to the workspace, part 2c (a tile that an
+// earlier block began) or 2c + 1 (one that a later block ends) of block c, and
+// cache_attention_join_kernel joins them.
 template <int ST, int D, int NQ>
-int run(const CacheAttnArgs& a, int64_t most_keys, cudaStream_t stream)
+__global__ void __launch_bounds__(kThreads) cache_attention_split_kernel(CacheAttnArgs a, float* part_o, float2* part_ml)
+{
+    using S = Step<ST, D>;
+    constexpr int kRows = 8 * NQ;
+    extern __shared__ __align__(128) char shared[];
+    __shared__ float2 ml_s[kWarps][kRows];
+    __shared__ Place place_s;
+    __shared__ int64_t total_s;
+    const int warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp == 0)
+    {
+        int64_t total = 0;
+        find_round<S>(a, kRows, 0, &total);
+        if (threadIdx.x == 0)
+            total_s = total;
+    }
+    __syncthreads();
+    const int64_t total = total_s;
+    const int n = dealt(total, gridDim.x), c = blockIdx.x;
+    if (c >= n)
+        return;
+    const float to_log2 = a.scale * 1.44269504088896341f;
+    const int64_t end = first_round(total, n, c + 1);
+    for (int64_t u = first_round(total, n, c); u < end;)
+    {
+        if (warp == 0)
+        {
+            const Place found = find_round<S>(a, kRows, u, nullptr);
+            if (threadIdx.x == 0)
+                place_s = found;
+        }
+        __syncthreads();
+        const Place place = place_s;
+        if (place.b < 0)
+            break;
+        const int64_t within = u - place.before;
+        const int which = (int)(within / place.r.per), round0 = (int)(within - (int64_t)which * place.r.per);
+        const int rounds = (int)min((int64_t)(place.r.per - round0), end - u);
+        Piece p;
+        p.kv = which / place.r.tiles;
+        p.tile = tile_of(a, place.b, which - p.kv * place.r.tiles, kRows, p.kv == 0 && round0 == 0 ? a.error_flag : nullptr);
+        p.first = tile_span(a, p.tile, 0);
+        p.last = tile_span(a, p.tile, p.tile.count - 1);
+        p.blocks = key_blocks(p.first, p.last, a.sinks, S::kKeys);
+        p.begin = round0 * kWarps;
+        p.end = min(p.blocks.count, (round0 + rounds) * kWarps);
+        WarpState<ST, D, NQ> w;
+        work<ST, D, NQ>(a, p, w, shared + warp * S::kWarpBytes, warp, kWarps);
+        float* parts_s = reinterpret_cast<float*>(shared);
+        publish<ST, D, NQ>(w, parts_s, ml_s);
+        const bool whole = rounds == place.r.per;
+        const int64_t slot = 2 * c + (round0 == 0 ? 1 : 0);
+        for (int e = threadIdx.x; e < p.tile.count * (D / 2); e += kThreads)
+        {
+            const int r = e / (D / 2), f = 2 * (e % (D / 2));
+            const Joined j = join(
+                kWarps, to_log2, [&](int i) { return ml_s[i][r]; },
+                [&](int i) { return *reinterpret_cast<const float2*>(parts_s + (i * kRows + r) * S::kPitch + f); });
+            if (whole)
+                store_out<D>(a, p.tile, p.kv, r, f, j);
+            else
+            {
+                *reinterpret_cast<float2*>(part_o + (slot * kRows + r) * D + f) = j.o;
+                if (f == 0)
+                    part_ml[slot * kRows + r] = make_float2(j.top, j.total);
+            }
+        }
+        __syncthreads();  // the shared memory becomes rings again
+        u += rounds;
+    }
+}
+
+// Joins the parts of the tiles that several blocks of cache_attention_split_kernel
+// (`blocks` of them) worked on. Blocks: x = tiles, y = heads, z = rows of a tile.
+template <int ST, int D, int NQ>
+__global__ void __launch_bounds__(D / 2) cache_attention_join_kernel(CacheAttnArgs a, int blocks, const float* part_o,
+                                                                   const float2* part_ml)
+{
+    using S = Step<ST, D>;
+    constexpr int kRows = 8 * NQ;
+    __shared__ QueryTile tile_s;
+    __shared__ Place place_s;
+    __shared__ int64_t total_s;
+    if (threadIdx.x < 32)
+    {
+        int64_t total = 0;
+        find_round<S>(a, kRows, 0, &total);
+        const QueryTile t = find_tile(a.mem, a.batch, a.group, kRows, blockIdx.x, nullptr);
+        // the first round of the sequence: all rounds of the sequences before it
+        int64_t before = 0;
+        if (t.b >= 0)
+            for (int base = 0; base < t.b; base += 32)
+            {
+                const int b = base + threadIdx.x;
+                const Rounds r = b < t.b ? sequence_rounds<S>(a, b, kRows) : Rounds{0, 0};
+                before += (int64_t)r.tiles * a.mem.heads * r.per;
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        if (threadIdx.x == 0)
+        {
+            total_s = total;
+            tile_s = t;
+            place_s.before = before;
+            place_s.r = t.b >= 0 ? sequence_rounds<S>(a, t.b, kRows) : Rounds{0, 0};
+        }
+    }
+    __syncthreads();
+    const QueryTile t = tile_s;
+    const int r = blockIdx.z, kv = blockIdx.y;
+    // every block, before anything else: the grid must not end ahead of the split kernel
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (t.b < 0 || r >= t.count)
+        return;
+    const int64_t total = total_s;
+    const int n = dealt(total, blocks);
+    const int per = place_s.r.per;
+    const int64_t u = place_s.before + ((int64_t)kv * place_s.r.tiles + t.m0 / kRows) * per;
+    // the block that has round v: the largest c with first_round(c) <= v
+    const auto block_of = [&](int64_t v) { return (int)(((v + 1) * n - 1) / total); };
+    const int c0 = block_of(u), c1 = block_of(u + per - 1);
+    if (c0 == c1)
+        return;  // finished by one block
+    const int f = 2 * threadIdx.x;
+    const auto slot = [&](int i) { return 2 * (int64_t)(c0 + i) + (i == 0 ? 1 : 0); };
+    const Joined j = join(
+        c1 - c0 + 1, a.scale * 1.44269504088896341f, [&](int i) { return part_ml[slot(i) * kRows + r]; },
+        [&](int i) { return *reinterpret_cast<const float2*>(part_o + (slot(i) * kRows + r) * D + f); });
+    store_out<D>(a, t, kv, r, f, j);
+}
+
+// Blocks of the split kernel: as many as run at once on 148 SMs.
+template <int ST, int D, int NQ>
+constexpr int split_blocks()
+{
+    const int by_memory = 232448 / (Step<ST, D>::shared_bytes(NQ) + 2048);
+    return 148 * (by_memory < 4 ? by_memory : 4);
+}
+
+template <int ST, int D, int NQ>
+constexpr size_t part_bytes()
+{
+    return (size_t)2 * split_blocks<ST, D, NQ>() * 8 * NQ * (D + 2) * 4;
+}
+
+template <int ST, int D, int NQ>
+int run(const CacheAttnArgs& a, int64_t most_keys, void* workspace, cudaStream_t stream)
 {
     using S = Step<ST, D>;
     const int64_t tiles = (int64_t)a.batch.rows * a.group / (8 * NQ) + a.batch.sequences;
-    // Blocks that share a tile's keys, at most 8 (the portable cluster size):
-    // as many as keep every SM busy to the end although sequences differ in
-    // length, as long as each warp still has some stages of its own.
-    int cluster = 1;
-    while (cluster < 8 && tiles * a.mem.heads * cluster < 148 * 8 && most_keys >= 4 * cluster * kWarps * S::kKeys)
-        cluster *= 2;
-    if (tiles * cluster > 0x7fffffff)
-        return (int)cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(tiles * cluster), (unsigned)a.mem.heads);
+    cudaLaunchAttribute attr = {};
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = S::shared_bytes(NQ);
     config.stream = stream;
-    cudaLaunchAttribute attr;
+    if (workspace)
+    {
+        const int blocks = split_blocks<ST, D, NQ>();
+        float* part_o = static_cast<float*>(workspace);
+        float2* part_ml = reinterpret_cast<float2*>(part_o + (size_t)2 * blocks * 8 * NQ * D);
+        config.gridDim = dim3((unsigned)blocks);
+        cudaError_t err = cudaLaunchKernelEx(&config, cache_attention_split_kernel<ST, D, NQ>, a, part_o, part_ml);
+        if (err != cudaSuccess)
+            return (int)err;
+        // starts while the split kernel runs and waits for its end on the device
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        config.gridDim = dim3((unsigned)tiles, (unsigned)a.mem.heads, 8 * NQ);
+        config.blockDim = dim3(D / 2);
+        config.dynamicSmemBytes = 0;
+        return (int)cudaLaunchKernelEx(&config, cache_attention_join_kernel<ST, D, NQ>, a, blocks,
+                                       (const float*)part_o, (const float2*)part_ml);
+    }
+    // Blocks that share a tile's keys, at most 8 (the portable cluster size):
+    // enough to fill the GPU, as long as each warp still has a key block or two.
+    int cluster = 1;
+    while (cluster < 8 && tiles * a.mem.heads * cluster < 148 * 4 && most_keys >= 2 * cluster * kWarps * S::kKeys)
+        cluster *= 2;
+    if (tiles * cluster > 0x7fffffff)
+        return (int)cudaErrorInvalidConfiguration;
+    config.gridDim = dim3((unsigned)(tiles * cluster), (unsigned)a.mem.heads);
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = cluster;
     attr.val.clusterDim.y = 1;
@@ -663,43 +1004,96 @@ int run(const CacheAttnArgs& a, int64_t most_keys, cudaStream_t stream)
     return (int)cudaLaunchKernelEx(&config, cache_attention_step_kernel<ST, D, NQ>, a, cluster);
 }
 
-template <int ST, int D>
-int run(const CacheAttnArgs& a, int max_rows, int64_t most_keys, cudaStream_t stream)
-{
-    return (int64_t)max_rows * a.group <= 8 ? run<ST, D, 1>(a, most_keys, stream) : run<ST, D, 2>(a, most_keys, stream);
-}
-
-template <int ST, int D>
+template <int ST, int D, int NQ>
 int prepare()
 {
-    cudaError_t err = cudaFuncSetAttribute(cache_attention_step_kernel<ST, D, 1>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize, Step<ST, D>::shared_bytes(1));
+    const int bytes = Step<ST, D>::shared_bytes(NQ);
+    cudaError_t err = cudaFuncSetAttribute(cache_attention_step_kernel<ST, D, NQ>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err == cudaSuccess)
-        err = cudaFuncSetAttribute(cache_attention_step_kernel<ST, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   Step<ST, D>::shared_bytes(2));
+        err = cudaFuncSetAttribute(cache_attention_split_kernel<ST, D, NQ>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     return (int)err;
 }
 
+// The kernel instance of a cache and a batch: F is called with its parameters.
+template <typename F>
+auto dispatch(int storage, int head_dim, bool two, F f)
+{
+    if (storage == AWA_INT4)
+        return head_dim == 64 ? (two ? f.template operator()<AWA_INT4, 64, 2>() : f.template operator()<AWA_INT4, 64, 1>())
+                              : (two ? f.template operator()<AWA_INT4, 128, 2>() : f.template operator()<AWA_INT4, 128, 1>());
+    return head_dim == 64 ? (two ? f.template operator()<AWA_BF16, 64, 2>() : f.template operator()<AWA_BF16, 64, 1>())
+                          : (two ? f.template operator()<AWA_BF16, 128, 2>() : f.template operator()<AWA_BF16, 128, 1>());
+}
+
+// Up to 8 (row, head) pairs per key/value head and sequence fit one tile of 8
+bool two_tiles(int group, int max_rows)
+{
+    return (int64_t)max_rows * group > 8;
+}
+
+struct WorkspaceOf
+{
+    int64_t most_keys;
+    template <int ST, int D, int NQ>
+    size_t operator()() const
+    {
+        // A cluster of 8 blocks gives each warp 4 key blocks of a cache this
+        // long: a launch alone is then most of the time
+        return most_keys <= 8 * kWarps * 4 * Step<ST, D>::kKeys ? 0 : part_bytes<ST, D, NQ>();
+    }
+};
+
+struct Run
+{
+    const CacheAttnArgs& a;
+    int64_t most_keys;
+    void* workspace;
+    cudaStream_t stream;
+    template <int ST, int D, int NQ>
+    int operator()() const
+    {
+        return run<ST, D, NQ>(a, most_keys, workspace, stream);
+    }
+};
+
+struct Prepare
+{
+    template <int ST, int D, int NQ>
+    int operator()() const
+    {
+        return prepare<ST, D, NQ>();
+    }
+};
+
 }  // namespace
 
-int launch_cache_attention_step(const CacheAttnArgs& a, int max_rows, int64_t most_keys, cudaStream_t stream)
+size_t cache_attention_step_workspace(const CacheMemory& mem, int group, int max_rows, int64_t most_keys)
+{
+    return dispatch(mem.storage, mem.head_dim, two_tiles(group, max_rows), WorkspaceOf{most_keys});
+}
+
+int launch_cache_attention_step(const CacheAttnArgs& a, int max_rows, int64_t most_keys, void* workspace,
+                                cudaStream_t stream)
 {
     ProfileScope scope("awa_cache_attention_step", stream);
-    if (a.mem.storage == AWA_INT4)
-        return a.mem.head_dim == 64 ? run<AWA_INT4, 64>(a, max_rows, most_keys, stream)
-                                    : run<AWA_INT4, 128>(a, max_rows, most_keys, stream);
-    return a.mem.head_dim == 64 ? run<AWA_BF16, 64>(a, max_rows, most_keys, stream)
-                                : run<AWA_BF16, 128>(a, max_rows, most_keys, stream);
+    if (!cache_attention_step_workspace(a.mem, a.group, max_rows, most_keys))
+        workspace = nullptr;
+    return dispatch(a.mem.storage, a.mem.head_dim, two_tiles(a.group, max_rows),
+                    Run{a, most_keys, workspace, stream});
 }
 
 int prepare_cache_attention_step()
 {
-    for (int (*set)() : {prepare<AWA_BF16, 64>, prepare<AWA_BF16, 128>, prepare<AWA_INT4, 64>, prepare<AWA_INT4, 128>})
-    {
-        const int err = set();
-        if (err)
-            return err;
-    }
+    for (int storage : {AWA_BF16, AWA_INT4})
+        for (int head_dim : {64, 128})
+            for (bool two : {false, true})
+            {
+                const int err = dispatch(storage, head_dim, two, Prepare{});
+                if (err)
+                    return err;
+            }
     return 0;
 }
 

@@ -149,10 +149,11 @@ __device__ __forceinline__ QueryTile find_tile(const CacheMemory& mem, const Cac
     for (int base = 0; base < batch.sequences; base += 32)
     {
         const int b = base + lane;
-        int start = 0, rows = 0;
+        int start = 0, rows = 0, past = 0;
         if (b < batch.sequences)
         {
             start = __ldg(batch.row_starts + b);
+            past = __ldg(batch.past + b);  // in flight with the starts
             rows = batch_rows(batch, b);
         }
         const int tiles = (int)(((int64_t)rows * group + tile - 1) / tile);
@@ -174,7 +175,7 @@ __device__ __forceinline__ QueryTile find_tile(const CacheMemory& mem, const Cac
             const int n = __shfl_sync(0xffffffffu, rows, src);
             t.m0 = (index - first) * tile;
             t.count = min(tile, n * group - t.m0);
-            t.past = max(0, __ldg(batch.past + t.b));
+            t.past = max(0, __shfl_sync(0xffffffffu, past, src));
             t.length = sequence_length(mem, batch, t.past, n, flag);
             t.past = min(t.past, t.length);  // of a cut sequence: keeps past + rows within 31 bits
             return t;

@@ -99,8 +99,11 @@ int launch_cache_unpack(const CacheUnpackArgs& args, int pages, cudaStream_t str
 // fp32 and bf16 caches of any head_dim, fp32 arithmetic.
 int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStream_t stream);
 // bf16 and 4-bit caches with head_dim 64 or 128, for few rows per sequence;
-// most_keys: no row sees more.
-int launch_cache_attention_step(const CacheAttnArgs& args, int max_rows, int64_t most_keys, cudaStream_t stream);
+// most_keys: no row sees more. The workspace holds the parts of tiles that
+// several blocks work on (0 bytes for short caches).
+size_t cache_attention_step_workspace(const CacheMemory& mem, int group, int max_rows, int64_t most_keys);
+int launch_cache_attention_step(const CacheAttnArgs& args, int max_rows, int64_t most_keys, void* workspace,
+                                cudaStream_t stream);
 // bf16 caches with head_dim 64 or 128 and at most 128 q heads per key/value
 // head, for many rows per sequence.
 int launch_cache_attention_tile(const CacheAttnArgs& args, cudaStream_t stream);

@@ -153,6 +153,9 @@ ATTEND = [
     ([1, 1, 1, 1], [0, 15, 16, 777], 16, 2, 8, 4, 100, 1),
     ([0, 1, 0, 3], [9, 40, 0, 130], 32, 1, 16, 0, 1, 1),    # window of one: each row itself
     ([1, 2], [5000, 3333], 128, 4, 4, 5, 1500, 1),
+    ([1, 1, 0, 2], [5000, 131, 40, 9000], 64, 2, 6, 4, 0, 1),  # long: the work dealt out over the blocks
+    ([4, 3, 1, 4], [6001, 17, 4500, 0], 32, 1, 8, 70, 6000, 1),  # two tiles a sequence
+    ([2], [12345], 256, 1, 1, 0, 0, 1),
     ([4, 2, 1], [60, 300, 0], 16, 2, 14, 17, 33, 1),        # prefix ends inside a page and a block
     ([17], [0], 16, 1, 1, 0, 0, 1),
     ([200], [0], 64, 2, 6, 0, 0, 1),
@@ -314,17 +317,19 @@ def test_frames_through_append_and_attention(storage):
 
 
 @pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
-def test_captured_step_serves_later_steps(storage):
+@pytest.mark.parametrize("width", [14, 1000])  # a table with room for long sequences takes other kernels
+def test_captured_step_serves_later_steps(width, storage):
     """One captured step of append and attention, replayed with other lengths,
     pages and rows, gives what eager calls give; two graphs may run at once."""
     dtype = torch.float32 if storage == "f32" else torch.bfloat16
     c = Batch([1, 1, 1], [207, 207, 207], 16, 2, 128, storage, seed=13)  # 13 pages each, of 41
+    c.table = torch.nn.functional.pad(c.table, (0, width - c.table.shape[1]), value=-1)
     cache, batch = c.handles(awa_b200)
     q, k, v = (c.new_rows(h, dtype) for h in (8, 2, 2))
     rope = awa_b200.CacheRope(awa_b200.rope_table(400, 64))
 
     def step():
-        return cache.attention(batch, cache.append(batch, k, v, q=q, rope=rope), sinks=4, window=50)
+        return cache.attention(batch, cache.append(batch, k, v, q=q, rope=rope), sinks=4, window=50 if width < 99 else 0)
 
     step()
     torch.cuda.synchronize()
@@ -354,10 +359,10 @@ def test_captured_step_serves_later_steps(storage):
 
 
 @pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
-@pytest.mark.parametrize("rows", [[1, 1], [70, 130]])
-def test_another_stream_and_repeatable(rows, storage):
+@pytest.mark.parametrize("rows,past", [([1, 1], [300, 40]), ([1, 2], [7000, 5500]), ([70, 130], [300, 40])])
+def test_another_stream_and_repeatable(rows, past, storage):
     dtype = torch.float32 if storage == "f32" else torch.bfloat16
-    c = Batch(rows, [300, 40], 16, 2, 128, storage, seed=14)
+    c = Batch(rows, past, 16, 2, 128, storage, seed=14)
     cache, batch = c.handles(awa_b200)
     q = c.new_rows(8, dtype)
     want = cache.attention(batch, q, sinks=4)
