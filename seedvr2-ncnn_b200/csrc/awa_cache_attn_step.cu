@@ -296,53 +296,93 @@ __device__ __forceinline__ int block_key(const Piece& p, int i)
     return (i < p.blocks.prefix ? i : i + p.blocks.shift) * S::kKeys;
 }
 
-// Issues the copies of key block i of the piece into stage `slot` of the warp's ring.
+// Copies 16 bytes that are all there.
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Page of a position of the piece's sequence; -1, reported, if there is none.
+__device__ __forceinline__ int piece_page(const CacheAttnArgs& a, const int* table, int key)
+{
+    const int page = __ldg(table + (key >> a.mem.page_shift));
+    if ((unsigned)page < (unsigned)a.mem.pages)
+        return page;
+    cache_error(a.error_flag, AWA_CACHE_BAD_PAGE);
+    return -1;
+}
+
+// Issues the copies of the key block at key0 into a stage of the warp's ring.
 template <int ST, int D>
-__device__ __forceinline__ void issue_block(const CacheAttnArgs& a, const Piece& p, int i, char* ring, int slot)
+__device__ __forceinline__ void issue_block(const CacheAttnArgs& a, const Piece& p, int key0, uint32_t dst)
 {
     using S = Step<ST, D>;
     const CacheMemory& mem = a.mem;
     const int lane = threadIdx.x & 31;
     const int* table = a.batch.page_table + p.tile.b * a.batch.table_stride;
     const int page_mask = (1 << mem.page_shift) - 1;
-    const int key0 = block_key<S>(p, i);
-    const uint32_t dst = shared_address(ring) + slot * S::kStageBytes;
-    // only what some row sees is read: pages outside may be gone
-    const auto seen = [&](int key) { return key < p.last.hi && (key >= p.first.lo || key < a.sinks); };
-    const bool all = key0 + S::kKeys <= p.last.hi && (key0 >= p.first.lo || key0 + S::kKeys <= a.sinks);
-    constexpr int kPieces = S::kRowBytes / 16;  // a power of two: 2, 4, 8 or 16
     const char* kbase = mem.k + p.kv * mem.head_stride;
     const char* vbase = mem.v + p.kv * mem.head_stride;
-#pragma unroll
-    for (int j = 0; j < S::kKeys * kPieces / 32; j++)
+    constexpr int kPieces = S::kRowBytes / 16;   // of a row, a power of two: 2, 4, 8 or 16
+    constexpr int kTurns = 16 * kPieces / 32;    // of a warp over 16 rows
+    constexpr int kValues = S::kKeys * S::kRowBytes;
+    int pages[S::kKeys / 16];  // 16 rows, aligned, lie in one page and are contiguous there
+    bool whole = key0 + S::kKeys <= p.last.hi && (key0 >= p.first.lo || key0 + S::kKeys <= a.sinks);
+    if (whole)
     {
-        const int r = (j * 32 + lane) / kPieces, c = (j * 32 + lane) % kPieces;
-        const int key = key0 + r;
-        bool real = all || seen(key);
-        int page = real ? __ldg(table + (key >> mem.page_shift)) : 0;
-        if ((unsigned)page >= (unsigned)mem.pages)
+#pragma unroll
+        for (int h = 0; h < S::kKeys / 16; h++)
+            pages[h] = piece_page(a, table, key0 + 16 * h);
+#pragma unroll
+        for (int h = 0; h < S::kKeys / 16; h++)
+            whole = whole && pages[h] >= 0;
+    }
+    if (whole)
+    {
+#pragma unroll
+        for (int h = 0; h < S::kKeys / 16; h++)
         {
-            cache_error(a.error_flag, AWA_CACHE_BAD_PAGE);
-            page = 0;
-            real = false;
+            const int64_t at =
+                pages[h] * mem.page_stride + ((key0 + 16 * h) & page_mask) * S::kRowBytes + 16 * lane;
+#pragma unroll
+            for (int j = 0; j < kTurns; j++)
+            {
+                const int r = 16 * h + (j * 32 + lane) / kPieces, c = (j * 32 + lane) % kPieces;
+                const uint32_t to = dst + piece_offset<ST, D>(r, c);
+                copy16(to, kbase + at + 512 * j);
+                copy16(to + kValues, vbase + at + 512 * j);
+            }
         }
-        const int64_t at = page * mem.page_stride + (int64_t)(key & page_mask) * S::kRowBytes + 16 * c;
-        const int to = piece_offset<ST, D>(r, c);
-        copy_async<16>(dst + to, kbase + at, real);
-        copy_async<16>(dst + S::kKeys * S::kRowBytes + to, vbase + at, real);
+    }
+    else
+    {
+        // only what some row sees is read: pages outside may be gone
+#pragma unroll
+        for (int j = 0; j < S::kKeys / 16 * kTurns; j++)
+        {
+            const int r = (j * 32 + lane) / kPieces, c = (j * 32 + lane) % kPieces;
+            const int key = key0 + r;
+            const bool seen = key < p.last.hi && (key >= p.first.lo || key < a.sinks);
+            const int page = seen ? piece_page(a, table, key) : -1;
+            const int64_t at = max(page, 0) * mem.page_stride + (int64_t)(key & page_mask) * S::kRowBytes + 16 * c;
+            const uint32_t to = dst + piece_offset<ST, D>(r, c);
+            copy_async<16>(to, kbase + at, page >= 0);
+            copy_async<16>(to + kValues, vbase + at, page >= 0);
+        }
     }
     if (S::kFour)
     {
         const int key = key0 + lane;
-        bool real = all || seen(key);
-        int page = real ? __ldg(table + (key >> mem.page_shift)) : 0;
-        real = real && (unsigned)page < (unsigned)mem.pages;
-        page = real ? page : 0;
-        const int64_t at = page * mem.params_page_stride + p.kv * mem.params_head_stride +
-                           (int64_t)(key & page_mask) * S::kParamBytes;
-        const uint32_t to = dst + 2 * S::kKeys * S::kRowBytes + lane * S::kParamBytes;
-        copy_async<S::kFour ? S::kParamBytes : 4>(to, mem.k_params + at, real);
-        copy_async<S::kFour ? S::kParamBytes : 4>(to + S::kKeys * S::kParamBytes, mem.v_params + at, real);
+        int page = -1;
+        if (whole)
+            page = lane < 16 ? pages[0] : pages[S::kKeys / 16 - 1];
+        else if (key < p.last.hi && (key >= p.first.lo || key < a.sinks))
+            page = piece_page(a, table, key);
+        const int64_t at = max(page, 0) * mem.params_page_stride + p.kv * mem.params_head_stride +
+                           (key & page_mask) * S::kParamBytes;
+        const uint32_t to = dst + 2 * kValues + lane * S::kParamBytes;
+        copy_async<S::kFour ? S::kParamBytes : 4>(to, mem.k_params + at, page >= 0);
+        copy_async<S::kFour ? S::kParamBytes : 4>(to + S::kKeys * S::kParamBytes, mem.v_params + at, page >= 0);
     }
 }
 
@@ -526,26 +566,26 @@ __device__ __forceinline__ void work(const CacheAttnArgs& a, const Piece& p, War
 {
     using S = Step<ST, D>;
     float2* scales = reinterpret_cast<float2*>(ring + kStages * S::kStageBytes);
-    const auto issue = [&](int n) {
-        const int i = p.begin + turn + n * turns;
+    const uint32_t ring_addr = shared_address(ring);
+    const auto issue = [&](int i, int stage) {
         if (i < p.end)
-            issue_block<ST, D>(a, p, i, ring, n % kStages);
+            issue_block<ST, D>(a, p, block_key<S>(p, i), ring_addr + stage * S::kStageBytes);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    int i = p.begin + turn;
 #pragma unroll
     for (int n = 0; n < kStages - 1; n++)
-        issue(n);
+        issue(i + n * turns, n);
     start<ST, D, NQ>(a, p, w);
-    for (int n = 0;; n++)
+    int stage = 0;
+    for (; i < p.end; i += turns)
     {
-        const int i = p.begin + turn + n * turns;
-        if (i >= p.end)
-            break;
-        issue(n + kStages - 1);
+        issue(i + (kStages - 1) * turns, stage == 0 ? kStages - 1 : stage - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
-        consume<ST, D, NQ>(a, p, w, block_key<S>(p, i), ring + (n % kStages) * S::kStageBytes, scales);
+        consume<ST, D, NQ>(a, p, w, block_key<S>(p, i), ring + stage * S::kStageBytes, scales);
         __syncwarp();  // the stage is free for the copies of the next round
+        stage = stage == kStages - 1 ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
