@@ -14,13 +14,16 @@
 // columns, so one row wastes 7/8 of the instruction instead of 15/16. The
 // running maximum and sum are those of the warp's keys, base 2, fp32.
 //
-// 4 bits: a code c stands for scale (c + z), z = minimum / scale. 128 + c is a
-// bf16 value whose bits are 0x4300 | c, so codes become operands with a shift
-// and a three-input logic operation, exactly. Per 64 features with their own scale,
-//   sum q k = scale (sum q (128 + c) + (z - 128) sum q)
-//   sum p v = sum p' (128 + c) + sum p' (z - 128),  p' = bf16(p scale),
-// the offsets in fp32, the second sum with the same rounded p', so that the
-// one rounding acts on p as it does for a bf16 cache.
+// 4 bits: a code c stands for scale (c + z), z = minimum / scale. As the bits
+// of a bf16 number, the integers 0..255 are the multiples of 2^-133 (the
+// subnormals and the binade above them), which mma.sync takes as they are: a
+// mask alone turns two codes of a word into an operand, one at bits 0-3 as
+// c 2^-133, one at bits 4-7 as 16 c 2^-133, exactly; the other operand carries
+// the powers of two that bring the products back. Per 64 features with their own scale,
+//   sum q k = scale (sum q c + z sum q)
+//   sum p v = sum p' c + sum p' z,  p' = bf16(p scale),
+// the sums in fp32, the last one with the same rounded p', so that the one
+// rounding acts on p as it does for a bf16 cache.
 #include "awa_cache_device.cuh"
 #include "awa_rows.cuh"
 
@@ -51,7 +54,7 @@ struct Step
     static constexpr int kKeys = kFour ? 32 : 2048 / D;
     static constexpr int kParamBytes = kFour ? 4 * kGroups : 0;
     static constexpr int kStageBytes = 2 * kKeys * (kRowBytes + kParamBytes);
-    // 4 bits: (scale, z - 128) of the stage's keys, [k, v][key][group]
+    // 4 bits: (scale, z) of the stage's keys, [k, v][key][group]; of the values, scale kProbsUp
     static constexpr int kScaleBytes = kFour ? 2 * kKeys * kGroups * 8 : 0;
     static constexpr int kWarpBytes = kStages * kStageBytes + kScaleBytes;
     static constexpr int kPitch = D + 4;  // floats of a row of partial results
@@ -112,10 +115,22 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Codes j and j + 4 of a word as the bf16 pair (128 + c_j, 128 + c_(j+4)).
+// Codes j and j + 4 of a word as the bits of two bf16 numbers: c 2^-133, for odd j 16 c 2^-133.
 __device__ __forceinline__ uint32_t code_pair(uint32_t word, int j)
 {
-    return ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+    return (word >> (8 * (j >> 1))) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
+}
+
+// The other operand's share of the powers of two. q 2^60 leaves q a range of
+// 2^67 up; p' 2^90 takes scales from about 2^-80 to 2^29.
+constexpr float kQueryUp = 0x1p60f, kScoresUp = 0x1p73f;
+constexpr float kProbsUp = 0x1p90f, kProbsDown = 0x1p-90f, kOutUp = 0x1p43f;
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t x, float f)
+{
+    uint32_t y;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(pack_bf16x2(f, f)));
+    return y;
 }
 
 // Where 16-byte piece c of row r of a stage lies. bf16: the 8 rows that one
@@ -148,7 +163,7 @@ struct WarpState
     uint32_t q[NQ][D / 16][2];  // Q^T operands
     float q_sum[NQ][S::kGroups][2];  // 4 bits: sum of q over a group, of columns 2t, 2t + 1
     float o[NQ][D / 16][4];
-    float off[NQ][S::kGroups][2];  // 4 bits: sum p' (z - 128)
+    float off[NQ][S::kGroups][2];  // 4 bits: sum p' z, times kProbsUp
     float top[NQ][2], sum[NQ][2];
     RowSpan span[NQ][2];
 };
@@ -203,7 +218,7 @@ __device__ __forceinline__ void scores(const WarpState<ST, D, NQ>& w, const char
             for (int c = 0; c < 4; c++)
             {
                 const float2 p = c < 2 ? p0 : p1;
-                const float part = fmaf(p.y, w.q_sum[n][gr][c & 1], acc[n][c]);
+                const float part = fmaf(p.y, w.q_sum[n][gr][c & 1], acc[n][c] * kScoresUp);
                 s[n][c] = gr == 0 ? p.x * part : fmaf(p.x, part, s[n][c]);
             }
     }
@@ -411,11 +426,11 @@ __device__ __forceinline__ void start(const CacheAttnArgs& a, const Piece& p, Wa
                     uint4 x = make_uint4(0, 0, 0, 0);
                     if (mine)
                         x = __ldg(reinterpret_cast<const uint4*>(row + 64 * gr + 16 * t + 8 * h));
-                    // pairs of features j, j + 4 as code_pair makes them
-                    w.q[n][4 * gr + 2 * h][0] = __byte_perm(x.x, x.z, 0x5410);
-                    w.q[n][4 * gr + 2 * h][1] = __byte_perm(x.x, x.z, 0x7632);
-                    w.q[n][4 * gr + 2 * h + 1][0] = __byte_perm(x.y, x.w, 0x5410);
-                    w.q[n][4 * gr + 2 * h + 1][1] = __byte_perm(x.y, x.w, 0x7632);
+                    // pairs of features j, j + 4 as code_pair makes them, odd j with its 16
+                    w.q[n][4 * gr + 2 * h][0] = mul_bf16x2(__byte_perm(x.x, x.z, 0x5410), kQueryUp);
+                    w.q[n][4 * gr + 2 * h][1] = mul_bf16x2(__byte_perm(x.x, x.z, 0x7632), kQueryUp / 16);
+                    w.q[n][4 * gr + 2 * h + 1][0] = mul_bf16x2(__byte_perm(x.y, x.w, 0x5410), kQueryUp);
+                    w.q[n][4 * gr + 2 * h + 1][1] = mul_bf16x2(__byte_perm(x.y, x.w, 0x7632), kQueryUp / 16);
                     const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int i = 0; i < 4; i++)
@@ -467,9 +482,9 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
     const char* vdata = kdata + S::kKeys * S::kRowBytes;
     if (S::kFour)
     {
-        // a lane works out (scale, z - 128) of its key. A scale of 0 or next
-        // to it (then the value is the minimum) is raised to where z and
-        // scale z stay finite: that moves the value by 15 * 2^-100 of it
+        // a lane works out (scale, z) of its key. A scale of 0 or next to it
+        // (then the value is the minimum) is raised to where z stays finite:
+        // that moves the value by at most 15 * 2^-80 of max(1, it)
         const uint32_t* par = reinterpret_cast<const uint32_t*>(vdata + S::kKeys * S::kRowBytes);
 #pragma unroll
         for (int x = 0; x < 2; x++)
@@ -478,8 +493,11 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
             {
                 const uint32_t word = par[(x * S::kKeys + lane) * S::kGroups + gr];
                 const float low = __uint_as_float(word & 0xffff0000u);
-                const float scale = fmaxf(__uint_as_float(word << 16), 0x1p-100f * fmaxf(1.f, fabsf(low)));
-                scales[(x * S::kKeys + lane) * S::kGroups + gr] = make_float2(scale, __fdividef(low, scale) - 128.f);
+                const float scale = fmaxf(__uint_as_float(word << 16), 0x1p-80f * fmaxf(1.f, fabsf(low)));
+                float inverse;  // scale is a normal number: 1 ulp, as a division's
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
+                scales[(x * S::kKeys + lane) * S::kGroups + gr] =
+                    make_float2(x == 0 ? scale : scale * kProbsUp, low * inverse);
             }
         __syncwarp();
     }
@@ -503,22 +521,22 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
                     if (!(key < span.hi && (key >= span.lo || key < a.sinks)))
                         s[b][x][c] = -INFINITY;
                 }
-    float base[NQ][2];
+    // The exponentials are taken from `top`, the largest score when it was last
+    // looked for: until one exceeds it by 8 (log2) they stay below 2^8, and the
+    // lanes need not meet.
+    const float slack = 8.f / to_log2;
+    float local[NQ][2];
     bool grew = false;
 #pragma unroll
     for (int x = 0; x < NQ; x++)
 #pragma unroll
         for (int c = 0; c < 2; c++)
         {
-            float top = fmaxf(s[0][x][c], s[0][x][c + 2]);
+            local[x][c] = fmaxf(s[0][x][c], s[0][x][c + 2]);
 #pragma unroll
             for (int b = 1; b < kBlocks; b++)
-                top = fmaxf(top, fmaxf(s[b][x][c], s[b][x][c + 2]));
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1)
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            base[x][c] = fmaxf(top, w.top[x][c]);
-            grew |= top > w.top[x][c];
+                local[x][c] = fmaxf(local[x][c], fmaxf(s[b][x][c], s[b][x][c + 2]));
+            grew |= local[x][c] > w.top[x][c] + slack;
         }
     if (__any_sync(0xffffffffu, grew))
 #pragma unroll
@@ -526,8 +544,12 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
 #pragma unroll
             for (int c = 0; c < 2; c++)
             {
-                const float old = w.top[x][c] == base[x][c] ? 1.f : fast_exp2((w.top[x][c] - base[x][c]) * to_log2);
-                w.top[x][c] = base[x][c];
+                float top = fmaxf(local[x][c], w.top[x][c]);
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1)
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                const float old = w.top[x][c] == top ? 1.f : fast_exp2((w.top[x][c] - top) * to_log2);
+                w.top[x][c] = top;
                 w.sum[x][c] *= old;
 #pragma unroll
                 for (int gr = 0; gr < S::kGroups; gr++)
@@ -545,7 +567,7 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
         for (int c = 0; c < 2; c++)
         {
             // nothing seen yet: all exponentials are 0
-            const float from = base[x][c] == -INFINITY ? 0.f : base[x][c] * to_log2;
+            const float from = w.top[x][c] == -INFINITY ? 0.f : w.top[x][c] * to_log2;
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
             {
@@ -668,7 +690,10 @@ __device__ __forceinline__ void publish(const WarpState<ST, D, NQ>& w, float* pa
                 for (int h = 0; h < 2; h++)
                 {
                     const int f = S::kFour ? 64 * (j / 4) + 8 * g + 4 * h + j % 4 : 16 * j + 8 * h + g;
-                    parts[(warp * 8 * NQ + r) * S::kPitch + f] = w.o[x][j][c + 2 * h] + (S::kFour ? off[j / 4] : 0.f);
+                    float o = w.o[x][j][c + 2 * h];
+                    if (S::kFour)
+                        o = fmaf(o, j & 1 ? kOutUp / 16 : kOutUp, off[j / 4] * kProbsDown);
+                    parts[(warp * 8 * NQ + r) * S::kPitch + f] = o;
                 }
         }
     __syncthreads();
