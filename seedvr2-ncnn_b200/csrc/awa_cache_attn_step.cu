@@ -40,7 +40,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 3;
+constexpr int kStages = 3;  // 2 leave too little in flight (4 bits: 177 us for 142), 4 too few blocks on an SM (163)
 
 // Sizes of one kernel instance.
 template <int ST, int D>
@@ -137,14 +137,17 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t x, float f)
 // ldmatrix reads fall on different banks. 4 bits (64-byte rows of two 32-byte
 // groups): the groups of half the rows swap places, so that neither the 8-byte
 // reads of keys nor the 4-byte reads of values collide.
+// The row is base + r, base a multiple of 8: its share is known when compiling.
 template <int ST, int D>
-__device__ __forceinline__ int piece_offset(int r, int c)
+__device__ __forceinline__ int piece_offset(int base, int r, int c)
 {
+    constexpr int kRowBytes = Step<ST, D>::kRowBytes;
+    int at = c;
     if (ST != AWA_INT4)
-        return r * 2 * D + ((c ^ (r & 7)) << 4);
-    if (D == 64)
-        return r * 32 + (c << 4);
-    return r * 64 + ((c ^ ((((r >> 1) ^ (r >> 2)) & 1) << 1)) << 4);
+        at = c ^ (r & 7);
+    else if (D == 128)
+        at = c ^ ((((r >> 1) ^ (r >> 2)) & 1) << 1);
+    return r * kRowBytes + (at << 4) + base * kRowBytes;
 }
 
 // The key that row r of a 16-key block holds. 4 bits: rows 2t, 2t + 1 (whose
@@ -156,12 +159,19 @@ __device__ __forceinline__ int key_of_row(int r)
     return ST == AWA_INT4 ? (r & 8) | ((r & 1) << 2) | ((r & 7) >> 1) : r;
 }
 
+// (scale, z) of the groups of a key, as the sums use them: with kScoresUp or kProbsUp.
+template <typename S>
+struct alignas(8 * S::kGroups) Scales
+{
+    float2 of[S::kGroups];
+};
+
 template <int ST, int D, int NQ>
 struct WarpState
 {
     using S = Step<ST, D>;
     uint32_t q[NQ][D / 16][2];  // Q^T operands
-    float q_sum[NQ][S::kGroups][2];  // 4 bits: sum of q over a group, of columns 2t, 2t + 1
+    float q_sum[NQ][S::kGroups][2];  // 4 bits: sum of q over a group over kScoresUp, of columns 2t, 2t + 1
     float o[NQ][D / 16][4];
     float off[NQ][S::kGroups][2];  // 4 bits: sum p' z, times kProbsUp
     float top[NQ][2], sum[NQ][2];
@@ -170,7 +180,8 @@ struct WarpState
 
 // The warp's share of one 16-key block: scores, exponentials, probabilities.
 template <int ST, int D, int NQ>
-__device__ __forceinline__ void scores(const WarpState<ST, D, NQ>& w, const char* kdata, const float2* kscale, int block,
+__device__ __forceinline__ void scores(const WarpState<ST, D, NQ>& w, const char* kdata,
+                                       const Scales<Step<ST, D>>* kscale, int block,
                                        float (&s)[NQ][4])
 {
     using S = Step<ST, D>;
@@ -180,27 +191,29 @@ __device__ __forceinline__ void scores(const WarpState<ST, D, NQ>& w, const char
 #pragma unroll
         for (int n = 0; n < NQ; n++)
             s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-        const int r = block * 16 + (lane & 15);
         const uint32_t base = shared_address(kdata);
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
         {
             uint32_t a[4];
-            ldmatrix_x4(base + piece_offset<ST, D>(r, 2 * i + (lane >> 4)), a);
+            ldmatrix_x4(base + piece_offset<ST, D>(block * 16, lane & 15, 2 * i + (lane >> 4)), a);
 #pragma unroll
             for (int n = 0; n < NQ; n++)
                 mma(s[n], a[0], a[1], a[2], a[3], w.q[n][i][0], w.q[n][i][1]);
         }
         return;
     }
-    const int r0 = block * 16 + key_of_row<ST>(g), r1 = r0 + 8;
+    const int r = key_of_row<ST>(g);  // and r + 8
+    const Scales<S> p0 = kscale[block * 16 + r], p1 = kscale[block * 16 + 8 + r];
 #pragma unroll
     for (int gr = 0; gr < S::kGroups; gr++)
     {
         float acc[NQ][4] = {};
         // 16 features of a lane: 8 bytes of each of its two keys
-        const uint2 x0 = *reinterpret_cast<const uint2*>(kdata + piece_offset<ST, D>(r0, 2 * gr) + 8 * t);
-        const uint2 x1 = *reinterpret_cast<const uint2*>(kdata + piece_offset<ST, D>(r1, 2 * gr) + 8 * t);
+        const uint2 x0 =
+            *reinterpret_cast<const uint2*>(kdata + piece_offset<ST, D>(block * 16, r, 2 * gr) + 8 * t);
+        const uint2 x1 =
+            *reinterpret_cast<const uint2*>(kdata + piece_offset<ST, D>(block * 16 + 8, r, 2 * gr) + 8 * t);
 #pragma unroll
         for (int i = 0; i < 4; i++)
         {
@@ -211,14 +224,13 @@ __device__ __forceinline__ void scores(const WarpState<ST, D, NQ>& w, const char
                 mma(acc[n], code_pair(a, j), code_pair(b, j), code_pair(a, j + 1), code_pair(b, j + 1),
                     w.q[n][4 * gr + i][0], w.q[n][4 * gr + i][1]);
         }
-        const float2 p0 = kscale[r0 * S::kGroups + gr], p1 = kscale[r1 * S::kGroups + gr];
 #pragma unroll
         for (int n = 0; n < NQ; n++)
 #pragma unroll
             for (int c = 0; c < 4; c++)
             {
-                const float2 p = c < 2 ? p0 : p1;
-                const float part = fmaf(p.y, w.q_sum[n][gr][c & 1], acc[n][c] * kScoresUp);
+                const float2 p = c < 2 ? p0.of[gr] : p1.of[gr];
+                const float part = fmaf(p.y, w.q_sum[n][gr][c & 1], acc[n][c]);
                 s[n][c] = gr == 0 ? p.x * part : fmaf(p.x, part, s[n][c]);
             }
     }
@@ -226,7 +238,8 @@ __device__ __forceinline__ void scores(const WarpState<ST, D, NQ>& w, const char
 
 // O^T += V^T P^T of one 16-key block; p: the exponentials in the layout of the scores.
 template <int ST, int D, int NQ>
-__device__ __forceinline__ void values(WarpState<ST, D, NQ>& w, const char* vdata, const float2* vscale, int block,
+__device__ __forceinline__ void values(WarpState<ST, D, NQ>& w, const char* vdata,
+                                       const Scales<Step<ST, D>>* vscale, int block,
                                        const float (&p)[NQ][4])
 {
     using S = Step<ST, D>;
@@ -240,25 +253,25 @@ __device__ __forceinline__ void values(WarpState<ST, D, NQ>& w, const char* vdat
             b[n][0] = transpose8x8(pack_bf16x2(p[n][0], p[n][1]));
             b[n][1] = transpose8x8(pack_bf16x2(p[n][2], p[n][3]));
         }
-        const int r = block * 16 + (lane & 7) + ((lane >> 4) << 3);
         const uint32_t base = shared_address(vdata);
+        const int r = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
         {
             uint32_t a[4];
-            ldmatrix_x4_trans(base + piece_offset<ST, D>(r, 2 * i + ((lane >> 3) & 1)), a);
+            ldmatrix_x4_trans(base + piece_offset<ST, D>(block * 16, r, 2 * i + ((lane >> 3) & 1)), a);
 #pragma unroll
             for (int n = 0; n < NQ; n++)
                 mma(w.o[n][i], a[0], a[1], a[2], a[3], b[n][0], b[n][1]);
         }
         return;
     }
-    const int r0 = block * 16 + key_of_row<ST>(g), r1 = r0 + 8;
-    const int k0 = block * 16 + t;  // keys of rows 2t, 2t + 1, 2t + 8, 2t + 9: k0, + 4, + 8, + 12
+    const int r = key_of_row<ST>(g);  // and r + 8
+    const Scales<S> s0 = vscale[block * 16 + r], s1 = vscale[block * 16 + 8 + r];
 #pragma unroll
     for (int gr = 0; gr < S::kGroups; gr++)
     {
-        const float2 p0 = vscale[r0 * S::kGroups + gr], p1 = vscale[r1 * S::kGroups + gr];
+        const float2 p0 = s0.of[gr], p1 = s1.of[gr];
         uint32_t b[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; n++)
@@ -272,11 +285,12 @@ __device__ __forceinline__ void values(WarpState<ST, D, NQ>& w, const char* vdat
             b[n][0] = transpose8x8(lo);
             b[n][1] = transpose8x8(hi);
         }
-        uint32_t x[4];  // features 8g .. 8g + 7 of the group, of the lane's four keys
+        // features 8g .. 8g + 7 of the group, of the keys of rows 2t, 2t + 1, 2t + 8, 2t + 9
+        uint32_t x[4];
 #pragma unroll
         for (int u = 0; u < 4; u++)
-            x[u] = *reinterpret_cast<const uint32_t*>(vdata + piece_offset<ST, D>(k0 + 4 * u, 2 * gr + (g >> 2)) +
-                                                      4 * (g & 3));
+            x[u] = *reinterpret_cast<const uint32_t*>(
+                vdata + piece_offset<ST, D>(block * 16 + 8 * (u >> 1), t + 4 * (u & 1), 2 * gr + (g >> 2)) + 4 * (g & 3));
         const uint32_t lo01 = __byte_perm(x[0], x[1], 0x5410), hi01 = __byte_perm(x[0], x[1], 0x7632);
         const uint32_t lo23 = __byte_perm(x[2], x[3], 0x5410), hi23 = __byte_perm(x[2], x[3], 0x7632);
         // tile i of the group: rows g = feature 8g + i, rows g + 8 = feature 8g + 4 + i
@@ -317,6 +331,28 @@ __device__ __forceinline__ void copy16(uint32_t dst, const char* src)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// Where the lane's share of the piece's keys comes from.
+struct Source
+{
+    const int* table;
+    const char *k, *v;  // of the head, at the lane's 16 bytes of a row run
+    const char *k_params, *v_params;
+};
+
+template <int ST, int D>
+__device__ __forceinline__ Source source_of(const CacheAttnArgs& a, const Piece& p)
+{
+    const CacheMemory& mem = a.mem;
+    const int lane = threadIdx.x & 31;
+    Source s;
+    s.table = a.batch.page_table + p.tile.b * a.batch.table_stride;
+    s.k = mem.k + p.kv * mem.head_stride + 16 * lane;
+    s.v = mem.v + p.kv * mem.head_stride + 16 * lane;
+    s.k_params = mem.k_params + p.kv * mem.params_head_stride;
+    s.v_params = mem.v_params + p.kv * mem.params_head_stride;
+    return s;
+}
+
 // Page of a position of the piece's sequence; -1, reported, if there is none.
 __device__ __forceinline__ int piece_page(const CacheAttnArgs& a, const int* table, int key)
 {
@@ -329,17 +365,15 @@ __device__ __forceinline__ int piece_page(const CacheAttnArgs& a, const int* tab
 
 // Issues the copies of the key block at key0 into a stage of the warp's ring.
 template <int ST, int D>
-__device__ __forceinline__ void issue_block(const CacheAttnArgs& a, const Piece& p, int key0, uint32_t dst)
+__device__ __forceinline__ void issue_block(const CacheAttnArgs& a, const Piece& p, const Source& src, int key0,
+                                            uint32_t dst)
 {
     using S = Step<ST, D>;
     const CacheMemory& mem = a.mem;
     const int lane = threadIdx.x & 31;
-    const int* table = a.batch.page_table + p.tile.b * a.batch.table_stride;
     const int page_mask = (1 << mem.page_shift) - 1;
-    const char* kbase = mem.k + p.kv * mem.head_stride;
-    const char* vbase = mem.v + p.kv * mem.head_stride;
     constexpr int kPieces = S::kRowBytes / 16;   // of a row, a power of two: 2, 4, 8 or 16
-    constexpr int kTurns = 16 * kPieces / 32;    // of a warp over 16 rows
+    constexpr int kRun = 32 / kPieces;           // rows that a warp copies at a time
     constexpr int kValues = S::kKeys * S::kRowBytes;
     int pages[S::kKeys / 16];  // 16 rows, aligned, lie in one page and are contiguous there
     bool whole = key0 + S::kKeys <= p.last.hi && (key0 >= p.first.lo || key0 + S::kKeys <= a.sinks);
@@ -347,42 +381,42 @@ __device__ __forceinline__ void issue_block(const CacheAttnArgs& a, const Piece&
     {
 #pragma unroll
         for (int h = 0; h < S::kKeys / 16; h++)
-            pages[h] = piece_page(a, table, key0 + 16 * h);
+            pages[h] = piece_page(a, src.table, key0 + 16 * h);
 #pragma unroll
         for (int h = 0; h < S::kKeys / 16; h++)
             whole = whole && pages[h] >= 0;
     }
+    const int c = lane % kPieces;
     if (whole)
     {
 #pragma unroll
         for (int h = 0; h < S::kKeys / 16; h++)
         {
-            const int64_t at =
-                pages[h] * mem.page_stride + ((key0 + 16 * h) & page_mask) * S::kRowBytes + 16 * lane;
+            const int64_t at = pages[h] * mem.page_stride + ((key0 + 16 * h) & page_mask) * S::kRowBytes;
 #pragma unroll
-            for (int j = 0; j < kTurns; j++)
+            for (int j = 0; j < 16 / kRun; j++)
             {
-                const int r = 16 * h + (j * 32 + lane) / kPieces, c = (j * 32 + lane) % kPieces;
-                const uint32_t to = dst + piece_offset<ST, D>(r, c);
-                copy16(to, kbase + at + 512 * j);
-                copy16(to + kValues, vbase + at + 512 * j);
+                const int base = 16 * h + j * kRun;  // of 8 rows or more, or within them
+                const uint32_t to = dst + piece_offset<ST, D>(base & ~7, (base & 7) + lane / kPieces, c);
+                copy16(to, src.k + at + 512 * j);
+                copy16(to + kValues, src.v + at + 512 * j);
             }
         }
     }
     else
     {
         // only what some row sees is read: pages outside may be gone
-#pragma unroll
-        for (int j = 0; j < S::kKeys / 16 * kTurns; j++)
+#pragma unroll 1
+        for (int base = 0; base < S::kKeys; base += kRun)
         {
-            const int r = (j * 32 + lane) / kPieces, c = (j * 32 + lane) % kPieces;
-            const int key = key0 + r;
+            const int r = base + lane / kPieces, key = key0 + r;
             const bool seen = key < p.last.hi && (key >= p.first.lo || key < a.sinks);
-            const int page = seen ? piece_page(a, table, key) : -1;
-            const int64_t at = max(page, 0) * mem.page_stride + (int64_t)(key & page_mask) * S::kRowBytes + 16 * c;
-            const uint32_t to = dst + piece_offset<ST, D>(r, c);
-            copy_async<16>(to, kbase + at, page >= 0);
-            copy_async<16>(to + kValues, vbase + at, page >= 0);
+            const int page = seen ? piece_page(a, src.table, key) : -1;
+            const int64_t at =
+                max(page, 0) * mem.page_stride + ((key & page_mask) - lane / kPieces) * (int64_t)S::kRowBytes;
+            const uint32_t to = dst + piece_offset<ST, D>(0, r, c);
+            copy_async<16>(to, src.k + at, page >= 0);
+            copy_async<16>(to + kValues, src.v + at, page >= 0);
         }
     }
     if (S::kFour)
@@ -392,12 +426,11 @@ __device__ __forceinline__ void issue_block(const CacheAttnArgs& a, const Piece&
         if (whole)
             page = lane < 16 ? pages[0] : pages[S::kKeys / 16 - 1];
         else if (key < p.last.hi && (key >= p.first.lo || key < a.sinks))
-            page = piece_page(a, table, key);
-        const int64_t at = max(page, 0) * mem.params_page_stride + p.kv * mem.params_head_stride +
-                           (key & page_mask) * S::kParamBytes;
+            page = piece_page(a, src.table, key);
+        const int64_t at = max(page, 0) * mem.params_page_stride + (key & page_mask) * S::kParamBytes;
         const uint32_t to = dst + 2 * kValues + lane * S::kParamBytes;
-        copy_async<S::kFour ? S::kParamBytes : 4>(to, mem.k_params + at, page >= 0);
-        copy_async<S::kFour ? S::kParamBytes : 4>(to + S::kKeys * S::kParamBytes, mem.v_params + at, page >= 0);
+        copy_async<S::kFour ? S::kParamBytes : 4>(to, src.k_params + at, page >= 0);
+        copy_async<S::kFour ? S::kParamBytes : 4>(to + S::kKeys * S::kParamBytes, src.v_params + at, page >= 0);
     }
 }
 
@@ -454,7 +487,7 @@ __device__ __forceinline__ void start(const CacheAttnArgs& a, const Piece& p, Wa
 #pragma unroll
             for (int c = 0; c < 2; c++)
             {
-                w.q_sum[n][gr][c] = ST == AWA_INT4 ? __shfl_sync(0xffffffffu, part[gr], 4 * (2 * t + c)) : 0.f;
+                w.q_sum[n][gr][c] = ST == AWA_INT4 ? __shfl_sync(0xffffffffu, part[gr], 4 * (2 * t + c)) / kScoresUp : 0.f;
                 w.off[n][gr][c] = 0.f;
             }
         }
@@ -474,7 +507,8 @@ __device__ __forceinline__ void start(const CacheAttnArgs& a, const Piece& p, Wa
 // One key block, arrived in the ring.
 template <int ST, int D, int NQ>
 __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, WarpState<ST, D, NQ>& w, int key0,
-                                        const char* kdata, float2* scales)
+                                        const char* kdata,
+                                        Scales<Step<ST, D>>* scales)
 {
     using S = Step<ST, D>;
     const int lane = threadIdx.x & 31, g = lane >> 2;
@@ -485,20 +519,27 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
         // a lane works out (scale, z) of its key. A scale of 0 or next to it
         // (then the value is the minimum) is raised to where z stays finite:
         // that moves the value by at most 15 * 2^-80 of max(1, it)
-        const uint32_t* par = reinterpret_cast<const uint32_t*>(vdata + S::kKeys * S::kRowBytes);
+        struct alignas(4 * S::kGroups) Words
+        {
+            uint32_t word[S::kGroups];
+        };
+        const Words* par = reinterpret_cast<const Words*>(vdata + S::kKeys * S::kRowBytes);
 #pragma unroll
         for (int x = 0; x < 2; x++)
+        {
+            const Words words = par[x * S::kKeys + lane];
+            Scales<S> out;
 #pragma unroll
             for (int gr = 0; gr < S::kGroups; gr++)
             {
-                const uint32_t word = par[(x * S::kKeys + lane) * S::kGroups + gr];
-                const float low = __uint_as_float(word & 0xffff0000u);
-                const float scale = fmaxf(__uint_as_float(word << 16), 0x1p-80f * fmaxf(1.f, fabsf(low)));
+                const float low = __uint_as_float(words.word[gr] & 0xffff0000u);
+                const float scale = fmaxf(__uint_as_float(words.word[gr] << 16), 0x1p-80f * fmaxf(1.f, fabsf(low)));
                 float inverse;  // scale is a normal number: 1 ulp, as a division's
                 asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
-                scales[(x * S::kKeys + lane) * S::kGroups + gr] =
-                    make_float2(x == 0 ? scale : scale * kProbsUp, low * inverse);
+                out.of[gr] = make_float2(scale * (x == 0 ? kScoresUp : kProbsUp), low * inverse);
             }
+            scales[x * S::kKeys + lane] = out;
+        }
         __syncwarp();
     }
     constexpr int kBlocks = S::kKeys / 16;
@@ -578,7 +619,7 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
         }
 #pragma unroll
     for (int b = 0; b < kBlocks; b++)
-        values<ST, D, NQ>(w, vdata, scales + S::kKeys * S::kGroups, b, s[b]);
+        values<ST, D, NQ>(w, vdata, scales + S::kKeys, b, s[b]);
 }
 
 // The warp's share of the piece: key blocks begin + turn, + turns, ...
@@ -587,11 +628,12 @@ __device__ __forceinline__ void work(const CacheAttnArgs& a, const Piece& p, War
                                      int turn, int turns)
 {
     using S = Step<ST, D>;
-    float2* scales = reinterpret_cast<float2*>(ring + kStages * S::kStageBytes);
+    Scales<S>* scales = reinterpret_cast<Scales<S>*>(ring + kStages * S::kStageBytes);
     const uint32_t ring_addr = shared_address(ring);
+    const Source src = source_of<ST, D>(a, p);
     const auto issue = [&](int i, int stage) {
         if (i < p.end)
-            issue_block<ST, D>(a, p, block_key<S>(p, i), ring_addr + stage * S::kStageBytes);
+            issue_block<ST, D>(a, p, src, block_key<S>(p, i), ring_addr + stage * S::kStageBytes);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     int i = p.begin + turn;
@@ -875,7 +917,7 @@ __device__ __forceinline__ QueryTile tile_of(const CacheAttnArgs& a, int b, int 
 // earlier block began) or 2c + 1 (one that a later block ends) of block c, and
 // cache_attention_join_kernel joins them.
 template <int ST, int D, int NQ>
-__global__ void __launch_bounds__(kThreads) cache_attention_split_kernel(CacheAttnArgs a, float* part_o, float2* part_ml)
+__global__ void __launch_bounds__(kThreads, ST == AWA_INT4 && NQ == 1 ? 3 : 2) cache_attention_split_kernel(CacheAttnArgs a, float* part_o, float2* part_ml)
 {
     using S = Step<ST, D>;
     constexpr int kRows = 8 * NQ;
