@@ -43,7 +43,9 @@ using bf16 = __nv_bfloat16;
 constexpr int kRows = 128;  // query rows of a tile
 constexpr int kKeys = 128;  // keys of a block
 constexpr int kMmaWarp = 8;
-constexpr int kThreads = 320;  // 10 warps: 65536 registers leave each thread 200, which the softmax needs
+constexpr int kTmaWarp = 9;
+constexpr int kThreads = 384;  // 3 warpgroups; the last one gives registers to the softmax (a thread holds 128 scores)
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;  // 8 * 208 + 4 * 80 <= 12 * 168 per lane
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kColS = 0;    // + 128 * tile
 constexpr uint32_t kColO = 256;  // + 128 * tile
@@ -60,7 +62,7 @@ struct Tile
 
     uint8_t q[2][kBytes];
     uint8_t ring[kStages][kBytes];
-    uint64_t q_full, full[kStages], empty[kStages], s_full[2], p_full[2], o_full[2], mma_done;
+    uint64_t q_full, full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], mma_done;
     uint32_t tmem_base;
     int abort;
     QueryTile job;
@@ -275,12 +277,12 @@ __device__ __forceinline__ void issue_qk(uint32_t tmem_s, uint32_t q_addr, uint3
 // O[128 x D] (+)= P[128 x 128] V[128 x D], P in TMEM, V MN-major: 8-key groups
 // 1024 bytes apart, panels of 64 features kPanelBytes apart.
 template <int D>
-__device__ __forceinline__ void issue_pv(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_addr, bool accumulate)
+__device__ __forceinline__ void issue_pv(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_addr, bool accumulate, int half)
 {
     const uint32_t idesc = tc::idesc_bf16_f32(128, D, true);
     const uint64_t v = tc::smem_desc_sw128(v_addr, Tile<D>::kPanelBytes, 1024);
 #pragma unroll
-    for (int s = 0; s < kKeys / 16; s++)
+    for (int s = half * kKeys / 32; s < (half + 1) * kKeys / 32; s++)
         tc::mma_ts(tmem_o, tmem_p + (uint32_t)(s * 8), v + (uint64_t)(s * (2048 >> 4)), idesc,
                    (accumulate || s > 0) ? 1u : 0u);
 }
@@ -330,19 +332,22 @@ __device__ void mma_role(const CacheAttnArgs& a, Tile<D>& sh, const Job& job, ui
             const bool pv = i >= 0 && takes_part(a, job, x, key0);
             if (pv)
             {
-                if (!warp_wait(&sh.p_full[x], p_phase[x], abort, a.error_flag, 84))
+                // the first half of the keys while the softmax works on the second
+#pragma unroll
+                for (int h = 0; h < 2 && ok; h++)
                 {
-                    ok = false;
-                    break;
+                    ok = warp_wait(&sh.p_full[x][h], p_phase[x], abort, a.error_flag, 84);
+                    tc::fence_after_sync();
+                    if (ok && lane == 0)
+                        issue_pv<D>(tmem + kColO + 128 * x, tmem + kColS + 128 * x, tc::smem_addr(sh.ring[v_stage]),
+                                    started[x], h);
                 }
+                if (!ok)
+                    break;
                 p_phase[x] ^= 1;
             }
-            tc::fence_after_sync();
             if (lane == 0)
             {
-                if (pv)
-                    issue_pv<D>(tmem + kColO + 128 * x, tmem + kColS + 128 * x, tc::smem_addr(sh.ring[v_stage]),
-                                started[x]);
                 // S of the next block overwrites P of this one: the MMAs of one
                 // thread execute in issue order. The commit covers the P V
                 // before it too: the softmax may scale O once the scores are in.
@@ -530,11 +535,14 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, const Job& job
                 pk[j] = pack_bf16x2(p0, p1);  // the operand type of P V; the sums keep fp32
             }
             tc::tmem_st16(t_s + 16 * c, pk);
+            if (c & 1)  // half of the keys
+            {
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                mbar_arrive(&sh.p_full[x][c >> 1]);
+            }
         }
         l_run = l_run * alpha + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
-        tc::tmem_wait_st();
-        tc::fence_before_sync();
-        mbar_arrive(&sh.p_full[x]);
     }
     if (!warp_wait(&sh.o_full[x], 0, abort, a.error_flag, 92))
         return;
@@ -599,7 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < 2; x++)
         {
             tc::mbar_init(&sh.s_full[x], 1);
-            tc::mbar_init(&sh.p_full[x], kRows);
+            tc::mbar_init(&sh.p_full[x][0], kRows);
+            tc::mbar_init(&sh.p_full[x][1], kRows);
             tc::mbar_init(&sh.o_full[x], 1);
         }
         tc::mbar_init(&sh.mma_done, 1);
@@ -621,11 +630,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = sh.tmem_base;
 
     if (warp < kMmaWarp)
+    {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         softmax_role<D>(a, sh, job, tmem);
-    else if (warp == kMmaWarp)
-        mma_role<D>(a, sh, job, tmem);
+    }
     else
-        tma_role<D>(a, maps, sh, job);
+    {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kMmaWarp)
+            mma_role<D>(a, sh, job, tmem);
+        else if (warp == kTmaWarp)
+            tma_role<D>(a, maps, sh, job);
+    }
 
     tc::fence_before_sync();
     __syncthreads();
