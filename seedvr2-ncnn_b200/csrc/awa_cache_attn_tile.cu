@@ -44,6 +44,7 @@ constexpr int kRows = 128;  // query rows of a tile
 constexpr int kKeys = 128;  // keys of a block
 constexpr int kMmaWarp = 8;
 constexpr int kTmaWarp = 9;
+constexpr int kCleanWarp = 10;
 constexpr int kThreads = 384;  // 3 warpgroups; the last one gives registers to the softmax (a thread holds 128 scores)
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;  // 8 * 208 + 4 * 80 <= 12 * 168 per lane
 constexpr uint32_t kTmemColumns = 512;
@@ -62,7 +63,9 @@ struct Tile
 
     uint8_t q[2][kBytes];
     uint8_t ring[kStages][kBytes];
-    uint64_t q_full, full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], mma_done;
+    static constexpr int kLanded = 8;  // at least the V copies in the ring
+
+    uint64_t q_full, full[kStages], empty[kStages], landed[kLanded], s_full[2], p_full[2][2], o_full[2], mma_done;
     uint32_t tmem_base;
     int abort;
     QueryTile job;
@@ -153,6 +156,8 @@ struct Job
     bool has_b;
     RowSpan first[2], last[2];  // of tile A, B
     KeyBlocks blocks;           // of both
+    // tile x takes part in the key blocks b < hi[x] with b >= lo[x] or b < sinks
+    int lo[2], hi[2], sinks;
 };
 
 __device__ __forceinline__ Job make_job(const CacheAttnArgs& a, const QueryTile& t)
@@ -170,24 +175,40 @@ __device__ __forceinline__ Job make_job(const CacheAttnArgs& a, const QueryTile&
     job.first[1] = job.has_b ? span(p0 + job.rows_per_tile) : job.first[0];
     job.last[1] = job.has_b ? span(p0 + (t.count - 1) / a.group) : job.last[0];
     job.blocks = key_blocks(job.first[0], job.last[1], a.sinks, kKeys);
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+    {
+        job.lo[x] = job.first[x].lo / kKeys;
+        job.hi[x] = x == 1 && !job.has_b ? 0 : (job.last[x].hi + kKeys - 1) / kKeys;
+    }
+    job.sinks = (a.sinks + kKeys - 1) / kKeys;
     return job;
 }
 
-__device__ __forceinline__ int block_key(const Job& job, int i)
+// Block i of the job's is block number ... of the sequence.
+__device__ __forceinline__ int block_of(const Job& job, int i)
 {
-    return (i < job.blocks.prefix ? i : i + job.blocks.shift) * kKeys;
+    return i < job.blocks.prefix ? i : i + job.blocks.shift;
 }
 
-// Whether some row of tile x sees a key of the block at key0.
-__device__ __forceinline__ bool takes_part(const CacheAttnArgs& a, const Job& job, int x, int key0)
+// Whether some row of tile x sees a key of block b of the sequence.
+__device__ __forceinline__ bool takes_part(const Job& job, int x, int b)
 {
-    return (x == 0 || job.has_b) && key0 < job.last[x].hi && (key0 + kKeys > job.first[x].lo || key0 < a.sinks);
+    return b < job.hi[x] && (b >= job.lo[x] || b < job.sinks);
 }
 
 // Whether some row of the job sees the key.
 __device__ __forceinline__ bool seen(const CacheAttnArgs& a, const Job& job, int key)
 {
     return key < job.last[1].hi && (key >= job.first[0].lo || key < a.sinks);
+}
+
+// Whether every key of block b of the sequence is seen by some row. The others,
+// at the ends of the prefix and the window, have slots that may hold anything.
+__device__ __forceinline__ bool all_seen(const CacheAttnArgs& a, const Job& job, int b)
+{
+    const int key0 = b * kKeys;
+    return key0 + kKeys <= job.last[1].hi && (key0 >= job.first[0].lo || key0 + kKeys <= a.sinks);
 }
 
 // ---------------------------------------------------------------- TMA warp
@@ -214,7 +235,7 @@ __device__ void tma_role(const CacheAttnArgs& a, const Maps& maps, Tile<D>& sh, 
     const int* table = a.batch.page_table + job.t.b * a.batch.table_stride;
     const auto lookup = [&](int i) {
         int page = a.mem.pages;  // past the last: the load brings zeros
-        const int key = block_key(job, i) + mine * piece;
+        const int key = block_of(job, i) * kKeys + mine * piece;
         if (i < job.blocks.count && mine < pieces && key < job.last[1].hi &&
             (key + piece > job.first[0].lo || key < a.sinks))
         {
@@ -228,12 +249,14 @@ __device__ void tma_role(const CacheAttnArgs& a, const Maps& maps, Tile<D>& sh, 
         return page;
     };
     int next = lookup(0);
-    int n = 0;  // blocks issued
+    int n = 0;       // copies issued
+    int ragged = 0;  // of them through the clean-up warp
     for (int i = 0; i < job.blocks.count; i++)
     {
         const int page = next;
         next = lookup(i + 1);
-        const int slot = (block_key(job, i) + mine * piece) & ((1 << a.mem.page_shift) - 1);
+        const int block = block_of(job, i);
+        const int slot = (block * kKeys + mine * piece) & ((1 << a.mem.page_shift) - 1);
         bool ok = true;
 #pragma unroll
         for (int v = 0; v < 2; v++, n++)
@@ -244,19 +267,60 @@ __device__ void tma_role(const CacheAttnArgs& a, const Maps& maps, Tile<D>& sh, 
                 ok = false;
                 break;
             }
+            // values with unseen slots reach the MMA through the clean-up warp
+            uint64_t* bar = &sh.full[stage];
+            if (v && !all_seen(a, job, block))
+                bar = &sh.landed[ragged++ % T::kLanded];
             if (lane == 0)
-                mbar_expect(&sh.full[stage], T::kBytes);
+                mbar_expect(bar, T::kBytes);
             __syncwarp();
             if (mine < pieces)
                 tma_load_4d(tc::smem_addr(sh.ring[stage] + panel * T::kPanelBytes + mine * piece * 128),
-                            v ? &maps.v : &maps.k, 64 * panel, slot, job.kv, page, &sh.full[stage]);
+                            v ? &maps.v : &maps.k, 64 * panel, slot, job.kv, page, bar);
         }
         if (!ok)
             break;
     }
     drain_bar(&sh.q_full, 0, a.error_flag, 74);
+    for (int k = 0; k < T::kLanded && k < ragged; k++)
+        drain_bar(&sh.landed[(ragged - 1 - k) % T::kLanded], ((ragged - 1 - k) / T::kLanded) & 1, a.error_flag, 75);
+    // (the full barrier of such a copy completes once the clean-up warp is through)
     for (int k = 0; k < T::kStages && k < n; k++)
         drain_bar(&sh.full[(n - 1 - k) % T::kStages], ((n - 1 - k) / T::kStages) & 1, a.error_flag, 75);
+}
+
+// ---------------------------------------------------------------- clean-up warp
+// Values in slots that no row sees become zeros: their probabilities are 0,
+// but 0 * NaN is NaN.
+template <int D>
+__device__ void clean_role(const CacheAttnArgs& a, Tile<D>& sh, const Job& job)
+{
+    using T = Tile<D>;
+    const int lane = threadIdx.x & 31;
+    volatile int* abort = &sh.abort;
+    int ragged = 0;
+    for (int i = 0; i < job.blocks.count; i++)
+    {
+        const int block = block_of(job, i);
+        if (all_seen(a, job, block))
+            continue;
+        const bool ok = warp_wait(&sh.landed[ragged % T::kLanded], (ragged / T::kLanded) & 1, abort, a.error_flag, 76);
+        ragged++;
+        const int stage = (2 * i + 1) % T::kStages;
+        if (ok)
+            for (int r = lane; r < kKeys; r += 32)
+                if (!seen(a, job, block * kKeys + r))
+#pragma unroll
+                    for (int c = 0; c < 8 * T::kPanels; c++)
+                        reinterpret_cast<uint4*>(sh.ring[stage] + (c >> 3) * T::kPanelBytes + r * 128)[c & 7] =
+                            make_uint4(0, 0, 0, 0);
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0)
+            mbar_arrive(&sh.full[stage]);
+        if (!ok)
+            return;
+    }
 }
 
 // ---------------------------------------------------------------- MMA warp
@@ -287,92 +351,91 @@ __device__ __forceinline__ void issue_pv(uint32_t tmem_o, uint32_t tmem_p, uint3
                    (accumulate || s > 0) ? 1u : 0u);
 }
 
+// One thread: between the MMAs of one tile and the other's there is nothing but
+// waits that are mostly over, so the tensor cores do not run dry.
 template <int D>
-__device__ void mma_role(const CacheAttnArgs& a, Tile<D>& sh, const Job& job, uint32_t tmem)
+__device__ void mma_issue(const CacheAttnArgs& a, Tile<D>& sh, const Job& job, uint32_t tmem)
 {
     using T = Tile<D>;
-    const int lane = threadIdx.x & 31;
     volatile int* abort = &sh.abort;
-    uint32_t p_phase[2] = {0, 0};
-    bool started[2] = {false, false};
     const int count = job.blocks.count;
-    bool ok = count == 0 || warp_wait(&sh.q_full, 0, abort, a.error_flag, 81);
-    // step i: O += P V of block i, S of block i + 1; block j's K is copy 2j, its V copy 2j + 1
-    for (int i = -1; i < count && ok; i++)
+    uint32_t p_phase = 0;   // bit x: of tile x
+    uint32_t started = 0;
+    if (count > 0 && !wait_bar(&sh.q_full, 0, abort, a.error_flag, 81))
+        return;
+    // copy 2i is K of block i, copy 2i + 1 its V
+    int k_stage = 0, v_stage = T::kStages - 1;
+    uint32_t k_phase = 0, v_phase = 1;
+    bool now[2] = {false, false};  // the tile takes part in block i
+    // step i: O += P V of block i, S of block i + 1
+    for (int i = -1; i < count; i++)
     {
-        const int v_stage = (2 * i + 1) % T::kStages, k_stage = (2 * i + 2) % T::kStages;
         const bool more = i + 1 < count;
-        const int key0 = i >= 0 ? block_key(job, i) : 0, next0 = more ? block_key(job, i + 1) : 0;
-        if (i >= 0)
-        {
-            if (!warp_wait(&sh.full[v_stage], ((2 * i + 1) / T::kStages) & 1, abort, a.error_flag, 82))
-                break;
-            // Slots that no row sees may hold anything, and 0 * NaN is NaN: their
-            // values become zeros. Only the blocks at the ends of the prefix and
-            // the window have such slots.
-            if (!(seen(a, job, key0) && seen(a, job, key0 + kKeys - 1) &&
-                  (key0 >= job.first[0].lo || key0 + kKeys <= a.sinks)))
-            {
-                for (int r = lane; r < kKeys; r += 32)
-                    if (!seen(a, job, key0 + r))
-#pragma unroll
-                        for (int c = 0; c < 8 * T::kPanels; c++)
-                            reinterpret_cast<uint4*>(sh.ring[v_stage] + (c >> 3) * T::kPanelBytes + r * 128)[c & 7] =
-                                make_uint4(0, 0, 0, 0);
-                tc::fence_async_smem();
-                __syncwarp();
-            }
-        }
-        if (more && !warp_wait(&sh.full[k_stage], ((2 * i + 2) / T::kStages) & 1, abort, a.error_flag, 83))
-            break;
-        // unrolled: p_phase and started stay in registers
+        const int next = more ? block_of(job, i + 1) : 0;
+        const bool then[2] = {more && takes_part(job, 0, next), more && takes_part(job, 1, next)};
+        if (i >= 0 && !wait_bar(&sh.full[v_stage], v_phase, abort, a.error_flag, 82))
+            return;
+        const uint32_t v_addr = tc::smem_addr(sh.ring[v_stage]), k_addr = tc::smem_addr(sh.ring[k_stage]);
+        bool k_here = !more;
 #pragma unroll
         for (int x = 0; x < 2; x++)
         {
-            const bool pv = i >= 0 && takes_part(a, job, x, key0);
-            if (pv)
+            const uint32_t t_s = tmem + kColS + 128 * x, t_o = tmem + kColO + 128 * x;
+            if (now[x])
             {
                 // the first half of the keys while the softmax works on the second
 #pragma unroll
-                for (int h = 0; h < 2 && ok; h++)
+                for (int h = 0; h < 2; h++)
                 {
-                    ok = warp_wait(&sh.p_full[x][h], p_phase[x], abort, a.error_flag, 84);
+                    if (!wait_bar(&sh.p_full[x][h], (p_phase >> x) & 1, abort, a.error_flag, 84))
+                        return;
                     tc::fence_after_sync();
-                    if (ok && lane == 0)
-                        issue_pv<D>(tmem + kColO + 128 * x, tmem + kColS + 128 * x, tc::smem_addr(sh.ring[v_stage]),
-                                    started[x], h);
+                    issue_pv<D>(t_o, t_s, v_addr, (started >> x) & 1, h);
                 }
-                if (!ok)
-                    break;
-                p_phase[x] ^= 1;
+                p_phase ^= 1u << x;
+                started |= 1u << x;
             }
-            if (lane == 0)
+            if (!k_here)
             {
-                // S of the next block overwrites P of this one: the MMAs of one
-                // thread execute in issue order. The commit covers the P V
-                // before it too: the softmax may scale O once the scores are in.
-                if (more && takes_part(a, job, x, next0))
-                {
-                    issue_qk<D>(tmem + kColS + 128 * x, tc::smem_addr(sh.q[x]), tc::smem_addr(sh.ring[k_stage]));
-                    tc::mma_commit(&sh.s_full[x]);
-                }
+                if (!wait_bar(&sh.full[k_stage], k_phase, abort, a.error_flag, 83))
+                    return;
+                k_here = true;
             }
-            started[x] |= pv;
-            __syncwarp();
+            // S of the next block overwrites P of this one: the MMAs of one
+            // thread execute in issue order. The commit covers the P V before
+            // it too: the softmax may scale O once the scores are in.
+            if (then[x])
+            {
+                issue_qk<D>(t_s, tc::smem_addr(sh.q[x]), k_addr);
+                tc::mma_commit(&sh.s_full[x]);
+            }
+            now[x] = then[x];
         }
-        if (ok && lane == 0)
-        {
-            if (i >= 0)
-                tc::mma_commit(&sh.empty[v_stage]);
-            if (more)
-                tc::mma_commit(&sh.empty[k_stage]);
-        }
-        __syncwarp();
+        if (i >= 0)
+            tc::mma_commit(&sh.empty[v_stage]);
+        if (more)
+            tc::mma_commit(&sh.empty[k_stage]);
+        const auto advance = [](int& stage, uint32_t& phase) {  // two copies on
+            stage += 2;
+            if (stage >= T::kStages)
+            {
+                stage -= T::kStages;
+                phase ^= 1;
+            }
+        };
+        advance(k_stage, k_phase);
+        advance(v_stage, v_phase);
     }
-    if (lane == 0)
+    tc::mma_commit(&sh.o_full[0]);
+    tc::mma_commit(&sh.o_full[1]);
+}
+
+template <int D>
+__device__ void mma_role(const CacheAttnArgs& a, Tile<D>& sh, const Job& job, uint32_t tmem)
+{
+    if ((threadIdx.x & 31) == 0)
     {
-        tc::mma_commit(&sh.o_full[0]);
-        tc::mma_commit(&sh.o_full[1]);
+        mma_issue<D>(a, sh, job, tmem);
         tc::mma_commit(&sh.mma_done);
     }
     __syncwarp();
@@ -454,8 +517,8 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, const Job& job
     bool any = false;
     for (int i = 0; i < job.blocks.count; i++)
     {
-        const int key0 = block_key(job, i);
-        if (!takes_part(a, job, x, key0))
+        const int block = block_of(job, i), key0 = block * kKeys;
+        if (!takes_part(job, x, block))
             continue;
         if (!warp_wait(&sh.s_full[x], phase, abort, a.error_flag, 91))
             return;
@@ -604,6 +667,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&sh.full[s], 1);
             tc::mbar_init(&sh.empty[s], 1);
         }
+        for (int s = 0; s < Tile<D>::kLanded; s++)
+            tc::mbar_init(&sh.landed[s], 1);
         for (int x = 0; x < 2; x++)
         {
             tc::mbar_init(&sh.s_full[x], 1);
@@ -641,6 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma_role<D>(a, sh, job, tmem);
         else if (warp == kTmaWarp)
             tma_role<D>(a, maps, sh, job);
+        else if (warp == kCleanWarp)
+            clean_role<D>(a, sh, job);
     }
 
     tc::fence_before_sync();
