@@ -340,11 +340,12 @@ enum Kernel
 // Up to 32 (row, head) pairs per key/value head and sequence the step kernel
 // reads the keys once or twice at memory speed and fills its instructions; the
 // tile kernel always computes 128 of them.
-static Kernel kernel_of(const awa::CacheMemory& mem, int group, int max_rows)
+static Kernel kernel_of(const awa::CacheMemory& mem, const awa_cache_batch& batch, int group)
 {
     if (mem.storage == AWA_F32 || (mem.head_dim != 64 && mem.head_dim != 128))
         return kSimt;
-    if ((int64_t)max_rows * group <= 32 || group > 128)
+    if ((int64_t)batch.max_rows * group <= 32 || group > 128 ||
+        batch.sequences > awa::cache_attention_tile_sequences())
         return kStep;
     return mem.storage == AWA_INT4 ? kUnpackTile : kTile;
 }
@@ -364,7 +365,7 @@ static int64_t most_pages(const awa::CacheMemory& mem, const awa::CacheBatch& ba
     return some < all ? some : all;
 }
 
-// The workspace of kUnpackTile: keys, values, page table, each on 256 bytes.
+// The workspace of kUnpackTile ahead of the tile kernel's: keys, values, page table, each on 256 bytes.
 struct Unpacked
 {
     int64_t pages;
@@ -392,14 +393,17 @@ size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cac
         check_attention(kWhat, cache, batch, q_heads, sinks, window, frame_tokens) || empty)
         return 0;
     const int group = q_heads / cache->mem.heads;
-    const Kernel kernel = kernel_of(cache->mem, group, batch->max_rows);
+    const Kernel kernel = kernel_of(cache->mem, *batch, group);
     if (kernel == kStep)
         return awa::cache_attention_step_workspace(cache->mem, group, batch->max_rows,
                                                    most_seen(cache->mem, *batch, sinks, window, frame_tokens));
-    if (kernel != kUnpackTile)
+    if (kernel == kSimt)
         return 0;
+    const size_t parts = awa::cache_attention_tile_workspace(cache->mem.head_dim);
+    if (kernel == kTile)
+        return parts;
     const Unpacked u = unpacked_of(cache->mem, b, sinks, window, frame_tokens);
-    return 2 * u.pool_bytes + u.table_bytes;
+    return 2 * u.pool_bytes + u.table_bytes + parts;
 }
 
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,
@@ -449,13 +453,13 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
     a.error_flag = cache->error_flag;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     int err = 0;
-    switch (kernel_of(a.mem, a.group, batch->max_rows))
+    switch (kernel_of(a.mem, *batch, a.group))
     {
     case kStep:
         err = awa::launch_cache_attention_step(a, batch->max_rows,
                                                most_seen(a.mem, *batch, sinks, window, frame_tokens), workspace, s);
         break;
-    case kTile: err = awa::launch_cache_attention_tile(a, s); break;
+    case kTile: err = awa::launch_cache_attention_tile(a, workspace, s); break;
     case kSimt: err = awa::launch_cache_attention_simt(a, batch->max_rows, s); break;
     case kUnpackTile:
     {
@@ -483,7 +487,7 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
         a.mem.head_stride = (int64_t)u.page_bytes / a.mem.heads;
         a.batch.page_table = unpack.table;
         a.batch.table_stride = a.batch.table_width;
-        err = awa::launch_cache_attention_tile(a, s);
+        err = awa::launch_cache_attention_tile(a, reinterpret_cast<char*>(unpack.table) + u.table_bytes, s);
         break;
     }
     }

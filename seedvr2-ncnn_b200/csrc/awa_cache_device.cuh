@@ -66,17 +66,12 @@ struct RowSpan
 __device__ __forceinline__ RowSpan row_span(int p, int length, int sinks, int window, int frame_tokens)
 {
     RowSpan s;
-    if (p < sinks)
-    {
-        const int64_t end = ((int64_t)(p / frame_tokens) + 1) * frame_tokens;
-        s.lo = 0;
-        s.hi = (int)min((int64_t)min(sinks, length), end);
-        return s;
-    }
-    const int f = (p - sinks) / frame_tokens;
-    const int64_t end = sinks + ((int64_t)f + 1) * frame_tokens;
-    s.hi = (int)min((int64_t)length, end);
-    s.lo = window > 0 && f >= window ? sinks + (f - window + 1) * frame_tokens : 0;
+    const bool prefix = p < sinks;
+    const int at = prefix ? p : p - sinks;
+    const int f = frame_tokens == 1 ? at : at / frame_tokens;  // a division is most of this function
+    const int64_t end = (prefix ? 0 : sinks) + ((int64_t)f + 1) * frame_tokens;
+    s.hi = (int)min((int64_t)(prefix ? min(sinks, length) : length), end);
+    s.lo = !prefix && window > 0 && f >= window ? sinks + (f - window + 1) * frame_tokens : 0;
     return s;
 }
 

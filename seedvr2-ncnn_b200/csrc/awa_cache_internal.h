@@ -106,7 +106,9 @@ int launch_cache_attention_step(const CacheAttnArgs& args, int max_rows, int64_t
                                 cudaStream_t stream);
 // bf16 caches with head_dim 64 or 128 and at most 128 q heads per key/value
 // head, for many rows per sequence.
-int launch_cache_attention_tile(const CacheAttnArgs& args, cudaStream_t stream);
+size_t cache_attention_tile_workspace(int head_dim);
+int cache_attention_tile_sequences();  // the most it takes
+int launch_cache_attention_tile(const CacheAttnArgs& args, void* workspace, cudaStream_t stream);
 // cudaFuncSetAttribute calls of the kernels, once per handle (not allowed to
 // fail later, inside a capture).
 int prepare_cache_attention_simt();
