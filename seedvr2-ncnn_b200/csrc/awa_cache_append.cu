@@ -6,7 +6,6 @@
 // scale and a minimum per 64 features). Nothing is read or written twice, so
 // memory bounds it: bytes = rows * (q + k + v in, q + k + v out).
 #include "awa_cache_device.cuh"
-#include "awa_rows.cuh"
 
 #include <cuda_bf16.h>
 
@@ -17,7 +16,8 @@ namespace
 
 using bf16 = __nv_bfloat16;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;     // of cache_unpack_kernel
+constexpr int kMaxThreads = 512;  // of the others
 constexpr int kMaxTileRows = 8;
 
 // Page number `index` of all that the sequences of the batch see, counted
@@ -142,6 +142,65 @@ __device__ __forceinline__ void dequantize8(uint32_t codes, uint32_t params, flo
         v[i] = __fadd_rn(__fmul_rn((float)((codes >> (4 * i)) & 15u), scale), minimum);
 }
 
+// 8 consecutive elements as they are loaded: raw 16-byte pieces where the rows
+// allow them, so that several heads' loads fit the registers.
+template <typename T, bool ALIGNED>
+struct Raw8
+{
+    float v[8];
+    __device__ __forceinline__ void load(const T* p)
+    {
+        get8<T, ALIGNED>(p, v);
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            x[i] = v[i];
+    }
+};
+
+template <>
+struct Raw8<bf16, true>
+{
+    uint4 w;
+    __device__ __forceinline__ void load(const bf16* p)
+    {
+        w = __ldg(reinterpret_cast<const uint4*>(p));
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const
+    {
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+        {
+            x[2 * i] = __uint_as_float(words[i] << 16);
+            x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
+        }
+    }
+};
+
+// (x0, x1) -> (x0 c - x1 s, x1 c + x0 s), every product and sum rounded: the
+// products two at a time (x1 (-s) is -(x1 s) exactly), the sums one by one, since
+// a sum of pairs behind them was contracted into fused operations.
+__device__ __forceinline__ void rotate_x2(float& x0, float& x1, float c, float s)
+{
+    float a0, a1, b0, b1;
+    asm("{\n\t.reg .b64 x, y, cc, ss;\n\t"
+        "mov.b64 x, {%4, %5};\n\t"
+        "mov.b64 y, {%5, %4};\n\t"
+        "mov.b64 cc, {%6, %6};\n\t"
+        "mov.b64 ss, {%7, %8};\n\t"
+        "mul.rn.f32x2 x, x, cc;\n\t"
+        "mul.rn.f32x2 y, y, ss;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t"
+        "mov.b64 {%2, %3}, y;\n\t}"
+        : "=f"(a0), "=f"(a1), "=f"(b0), "=f"(b1)
+        : "f"(x0), "f"(x1), "f"(c), "f"(-s), "f"(s));
+    x0 = __fadd_rn(a0, b0);
+    x1 = __fadd_rn(a1, b1);
+}
+
 // A row of the batch: where it goes and how it turns.
 struct RowPlace
 {
@@ -151,36 +210,34 @@ struct RowPlace
     int coord[4];
 };
 
-// ST: the cache's storage type. Blocks: x = tiles of `tile_rows` rows, y =
-// parts of the heads. A thread keeps its 8 features (and so, within a row, its
-// rotation factors) and walks over the heads of q, k and v.
-template <typename TIn, typename TQ, int ST, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendArgs a, int tile_rows)
+// The places of the block's rows; a block barrier ends it. coords, table: of
+// the rotation, NULL without one.
+template <int ST>
+__device__ __forceinline__ void find_places(const CacheMemory& mem, const CacheBatch& batch, int row0, int rows,
+                                            const int* coords, bool rotates, int axes, int max_coord, int* flag,
+                                            RowPlace* places)
 {
-    __shared__ RowPlace places[kMaxTileRows];
-    const CacheMemory& mem = a.mem;
-    const int row0 = blockIdx.x * tile_rows;
-    if ((int)threadIdx.x < tile_rows)
+    if ((int)threadIdx.x < rows)
     {
-        RowPlace p;
+        RowPlace& p = places[threadIdx.x];
         p.position = -1;
         const int row = row0 + threadIdx.x;
-        const int b = row < a.batch.rows ? sequence_of_row(a.batch, row) : -1;
+        const int b = row < batch.rows ? sequence_of_row(batch, row) : -1;
         if (b >= 0)
         {
-            const int position = position_of_row(a.batch, b, row);
-            const int page = page_of(mem, a.batch, b, position, a.error_flag);
+            const int position = position_of_row(batch, b, row);
+            const int page = page_of(mem, batch, b, position, flag);
             bool good = page >= 0;
-            if (a.table)
-                for (int x = 0; x < a.axes; x++)
+            for (int x = 0; rotates && x < axes; x++)
+            {
+                const int c = coords ? __ldg(coords + (int64_t)row * axes + x) : position;
+                p.coord[x] = c;
+                if (c < 0 || c >= max_coord)
                 {
-                    p.coord[x] = a.coords ? __ldg(a.coords + (int64_t)row * a.axes + x) : position;
-                    if (p.coord[x] < 0 || p.coord[x] >= a.max_coord)
-                    {
-                        cache_error(a.error_flag, AWA_CACHE_BAD_COORD);
-                        good = false;
-                    }
+                    cache_error(flag, AWA_CACHE_BAD_COORD);
+                    good = false;
                 }
+            }
             if (good)
             {
                 const int slot = position & ((1 << mem.page_shift) - 1);
@@ -190,20 +247,60 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendArgs 
                 p.position = position;
             }
         }
-        places[threadIdx.x] = p;
     }
     __syncthreads();
+}
+
+// ST: the cache's storage type. A block takes tile_rows rows: `lanes` heads side
+// by side, head_dim / 8 threads each. A thread keeps its 8 features, and so,
+// within a row, its rotation factors, and takes every lanes-th head of q, k and v.
+template <typename TIn, typename TQ, int ST, bool ALIGNED>
+__global__ void __launch_bounds__(kMaxThreads, 2) cache_append_kernel(CacheAppendArgs a, int tile_rows, int lanes)
+{
+    __shared__ RowPlace places[kMaxTileRows];
+    const CacheMemory& mem = a.mem;
+    const int row0 = blockIdx.x * tile_rows;
+    find_places<ST>(mem, a.batch, row0, tile_rows, a.coords, a.table != nullptr, a.axes, a.max_coord, a.error_flag,
+                    places);
 
     const int chunks = mem.head_dim / 8;
-    const int lanes = kThreads / chunks;  // heads side by side
-    const int chunk = threadIdx.x % chunks, lane = threadIdx.x / chunks;
+    const int lane = threadIdx.x / chunks, chunk = threadIdx.x - lane * chunks;
     const int f = chunk * 8;
-    const int total = a.q_heads + 2 * mem.heads;
-    const int step = lanes * gridDim.y;
-    const TIn* q = reinterpret_cast<const TIn*>(a.q);
-    const TIn* k = reinterpret_cast<const TIn*>(a.k);
-    const TIn* v = reinterpret_cast<const TIn*>(a.v);
-    TQ* q_out = reinterpret_cast<TQ*>(a.q_out);
+    const int pairs = a.table ? a.axes * a.pairs : 0;
+    const int turned = min(4, max(0, pairs - f / 2));  // of this thread's pairs
+    const bool exists = lane < lanes;                  // the last warp may be longer than the heads
+    const TIn* q = reinterpret_cast<const TIn*>(a.q) + f;
+    const TIn* k = reinterpret_cast<const TIn*>(a.k) + f;
+    const TIn* v = reinterpret_cast<const TIn*>(a.v) + f;
+
+    const auto turn = [&](float(&x)[8], const float2(&cs)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < turned)
+                rotate_x2(x[2 * i], x[2 * i + 1], cs[i].x, cs[i].y);
+    };
+    const auto keep = [&](char* pages, char* params, const RowPlace& place, int h, bool mine, const float(&x)[8]) {
+        char* dst = pages + place.slot + h * mem.head_stride;
+        if (ST == AWA_INT4)
+        {
+            uint32_t codes, par;
+            quantize8(x, codes, par);  // all lanes: the groups' threads meet
+            if (mine)
+            {
+                *reinterpret_cast<uint32_t*>(dst + f / 2) = codes;
+                if (chunk % 8 == 0)
+                    *reinterpret_cast<uint32_t*>(params + place.params + h * mem.params_head_stride +
+                                                 f / AWA_CACHE_GROUP * 4) = par;
+            }
+        }
+        else if (mine)
+        {
+            if (ST == AWA_F32)
+                store8(reinterpret_cast<float*>(dst) + f, x);
+            else
+                store8(reinterpret_cast<bf16*>(dst) + f, x);
+        }
+    };
 
     for (int r = 0; r < tile_rows; r++)
     {
@@ -211,98 +308,69 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(CacheAppendArgs 
         if (place.position < 0)
             continue;
         const int64_t row = row0 + r;
+        const TIn* qr = q + row * a.q_stride;
+        const TIn* kr = k + row * a.k_stride;
+        const TIn* vr = v + row * a.v_stride;
+        TQ* out = reinterpret_cast<TQ*>(a.q_out) + row * a.q_out_stride + f;
+        // the loads of the first head of each kind ahead of the first use
+        Raw8<TIn, ALIGNED> q8 = {}, k8 = {}, v8 = {};
+        if (lane < a.q_heads && exists)
+            q8.load(qr + lane * mem.head_dim);
+        if (lane < mem.heads && exists)
+        {
+            k8.load(kr + lane * mem.head_dim);
+            v8.load(vr + lane * mem.head_dim);
+        }
         float2 cs[4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
         {
             cs[i] = make_float2(1.f, 0.f);
-            const int pair = f / 2 + i;
-            if (a.table && pair < a.axes * a.pairs)
+            if (i < turned)
             {
-                const int axis = pair / a.pairs;
+                const int pair = f / 2 + i;
+                const int axis = pair < a.pairs ? 0 : pair / a.pairs;
                 cs[i] = __ldg(a.table + (int64_t)place.coord[axis] * a.pairs + (pair - axis * a.pairs));
             }
         }
-        const bool turns = a.table && f < 2 * a.axes * a.pairs;
-        // uniform trip count: quantize8 shuffles within the warp
-        for (int h0 = blockIdx.y * lanes; h0 < total; h0 += step)
+        float x[8];
+        for (int h = lane; h < a.q_heads && exists; h += lanes)
+        {
+            q8.floats(x);
+            if (h + lanes < a.q_heads)
+                q8.load(qr + (h + lanes) * mem.head_dim);
+            turn(x, cs);
+            put8<TQ, ALIGNED>(out + h * mem.head_dim, x);
+        }
+        for (int h0 = 0; h0 < mem.heads; h0 += lanes)  // the same count in all threads
         {
             const int h = h0 + lane;
-            const bool mine = lane < lanes && h < total;
-            float x[8] = {};
-            const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + mem.heads;
-            if (mine)
+            const bool mine = h < mem.heads && exists, more = h + lanes < mem.heads && exists;
+            float y[8];
+            k8.floats(x);
+            v8.floats(y);
+            if (more)
             {
-                const TIn* src = is_q   ? q + row * a.q_stride + h * mem.head_dim
-                                 : is_k ? k + row * a.k_stride + (h - a.q_heads) * mem.head_dim
-                                        : v + row * a.v_stride + (h - a.q_heads - mem.heads) * mem.head_dim;
-                get8<TIn, ALIGNED>(src + f, x);
-                if (turns && (is_q || is_k))
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (f / 2 + i < a.axes * a.pairs)
-                            rope_rotate(x[2 * i], x[2 * i + 1], cs[i].x, cs[i].y, x[2 * i], x[2 * i + 1]);
+                k8.load(kr + (h + lanes) * mem.head_dim);
+                v8.load(vr + (h + lanes) * mem.head_dim);
             }
-            if (mine && is_q)
-                put8<TQ, ALIGNED>(q_out + row * a.q_out_stride + h * mem.head_dim + f, x);
-            const int kv = is_k ? h - a.q_heads : h - a.q_heads - mem.heads;
-            char* base = is_k ? mem.k : mem.v;
-            if (ST == AWA_INT4)
-            {
-                uint32_t codes, params;
-                quantize8(x, codes, params);
-                if (mine && !is_q)
-                {
-                    *reinterpret_cast<uint32_t*>(base + place.slot + kv * mem.head_stride + f / 2) = codes;
-                    if (chunk % 8 == 0)
-                        *reinterpret_cast<uint32_t*>((is_k ? mem.k_params : mem.v_params) + place.params +
-                                                     kv * mem.params_head_stride + f / AWA_CACHE_GROUP * 4) = params;
-                }
-            }
-            else if (mine && !is_q)
-            {
-                char* dst = base + place.slot + kv * mem.head_stride;
-                if (ST == AWA_F32)
-                    store8(reinterpret_cast<float*>(dst) + f, x);
-                else
-                    store8(reinterpret_cast<bf16*>(dst) + f, x);
-            }
+            turn(x, cs);
+            keep(mem.k, mem.k_params, place, h, mine, x);
+            keep(mem.v, mem.v_params, place, h, mine, y);
         }
     }
 }
 
 template <typename TOut, int ST, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheReadArgs a, int tile_rows)
+__global__ void __launch_bounds__(kMaxThreads, 2) cache_read_kernel(CacheReadArgs a, int tile_rows, int lanes)
 {
     __shared__ RowPlace places[kMaxTileRows];
     const CacheMemory& mem = a.mem;
     const int row0 = blockIdx.x * tile_rows;
-    if ((int)threadIdx.x < tile_rows)
-    {
-        RowPlace p;
-        p.position = -1;
-        const int row = row0 + threadIdx.x;
-        const int b = row < a.batch.rows ? sequence_of_row(a.batch, row) : -1;
-        if (b >= 0)
-        {
-            const int position = position_of_row(a.batch, b, row);
-            const int page = page_of(mem, a.batch, b, position, a.error_flag);
-            if (page >= 0)
-            {
-                const int slot = position & ((1 << mem.page_shift) - 1);
-                const int row_bytes = ST == AWA_INT4 ? mem.head_dim / 2 : mem.head_dim * (ST == AWA_F32 ? 4 : 2);
-                p.slot = page * mem.page_stride + (int64_t)slot * row_bytes;
-                p.params = page * mem.params_page_stride + (int64_t)slot * (mem.head_dim / AWA_CACHE_GROUP) * 4;
-                p.position = position;
-            }
-        }
-        places[threadIdx.x] = p;
-    }
-    __syncthreads();
+    find_places<ST>(mem, a.batch, row0, tile_rows, nullptr, false, 0, 0, a.error_flag, places);
 
     const int chunks = mem.head_dim / 8;
-    const int lanes = kThreads / chunks;
-    const int f = (threadIdx.x % chunks) * 8, lane = threadIdx.x / chunks;
+    const int lane = threadIdx.x / chunks, f = (threadIdx.x - lane * chunks) * 8;
     if (lane >= lanes)
         return;
     for (int r = 0; r < tile_rows; r++)
@@ -311,26 +379,34 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheReadArgs a, i
         if (place.position < 0)
             continue;
         const int64_t row = row0 + r;
-        for (int h = blockIdx.y * lanes + lane; h < 2 * mem.heads; h += lanes * gridDim.y)
+        TOut* k = reinterpret_cast<TOut*>(a.k_out) + row * a.k_stride + f;
+        TOut* v = reinterpret_cast<TOut*>(a.v_out) + row * a.v_stride + f;
+        for (int h = lane; h < mem.heads; h += lanes)
         {
-            const bool is_k = h < mem.heads;
-            const int kv = is_k ? h : h - mem.heads;
-            const char* src = (is_k ? mem.k : mem.v) + place.slot + kv * mem.head_stride;
-            float x[8];
+            const int64_t at = place.slot + h * mem.head_stride;
+            float x[8], y[8];
             if (ST == AWA_INT4)
             {
-                const uint32_t params =
-                    *reinterpret_cast<const uint32_t*>((is_k ? mem.k_params : mem.v_params) + place.params +
-                                                       kv * mem.params_head_stride + f / AWA_CACHE_GROUP * 4);
-                dequantize8(*reinterpret_cast<const uint32_t*>(src + f / 2), params, x);
+                const int64_t par = place.params + h * mem.params_head_stride + f / AWA_CACHE_GROUP * 4;
+                const uint32_t kc = *reinterpret_cast<const uint32_t*>(mem.k + at + f / 2);
+                const uint32_t vc = *reinterpret_cast<const uint32_t*>(mem.v + at + f / 2);
+                const uint32_t kp = *reinterpret_cast<const uint32_t*>(mem.k_params + par);
+                const uint32_t vp = *reinterpret_cast<const uint32_t*>(mem.v_params + par);
+                dequantize8(kc, kp, x);
+                dequantize8(vc, vp, y);
             }
             else if (ST == AWA_F32)
-                load8(reinterpret_cast<const float*>(src) + f, x);
+            {
+                load8(reinterpret_cast<const float*>(mem.k + at) + f, x);
+                load8(reinterpret_cast<const float*>(mem.v + at) + f, y);
+            }
             else
-                load8(reinterpret_cast<const bf16*>(src) + f, x);
-            TOut* dst = reinterpret_cast<TOut*>(is_k ? a.k_out : a.v_out) + row * (is_k ? a.k_stride : a.v_stride) +
-                        (int64_t)kv * mem.head_dim + f;
-            put8<TOut, ALIGNED>(dst, x);
+            {
+                load8(reinterpret_cast<const bf16*>(mem.k + at) + f, x);
+                load8(reinterpret_cast<const bf16*>(mem.v + at) + f, y);
+            }
+            put8<TOut, ALIGNED>(k + h * mem.head_dim, x);
+            put8<TOut, ALIGNED>(v + h * mem.head_dim, y);
         }
     }
 }
@@ -394,31 +470,43 @@ __global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs 
 
 struct Shape
 {
-    dim3 grid;
-    int tile_rows;
+    int blocks, threads, tile_rows, lanes;
 };
 
-// Few rows: a block per row and part of the heads (a step of 8 rows with 60
-// heads of 128 features fills 32 blocks). Many rows: a block takes 8 of them
-// whole, so the lookup of sequence, page and coordinates is paid once a tile.
-Shape shape_of(int rows, int heads, int head_dim)
+// Heads side by side: the multiple of the cache's heads that leaves the fewest
+// threads idle over q, k and v, at 128 to 512 threads. Few rows: a block each.
+// Many: a block takes 8, so the lookup of sequence, page and coordinates is paid
+// once a tile.
+Shape shape_of(int rows, int q_heads, int heads, int head_dim)
 {
     Shape s;
+    const int chunks = head_dim / 8, most = kMaxThreads / chunks, least = 128 / chunks + 1;
+    s.lanes = most;
+    double best = 0;
+    for (int lanes = heads < most ? heads : most; lanes <= most; lanes += heads)
+    {
+        const int passes = (q_heads + lanes - 1) / lanes + 2 * ((heads + lanes - 1) / lanes);
+        const double used = (double)(q_heads + 2 * heads) / ((double)passes * lanes);
+        if ((lanes >= least || lanes + heads > most) && used >= best)
+        {
+            best = used;
+            s.lanes = lanes;
+        }
+    }
+    s.threads = (s.lanes * chunks + 31) / 32 * 32;
     s.tile_rows = rows < 148 * 8 ? 1 : kMaxTileRows;
-    const int lanes = kThreads / (head_dim / 8);
-    const int passes = (heads + lanes - 1) / lanes;
-    s.grid = dim3((unsigned)((rows + s.tile_rows - 1) / s.tile_rows), s.tile_rows == 1 ? (unsigned)passes : 1u);
+    s.blocks = (rows + s.tile_rows - 1) / s.tile_rows;
     return s;
 }
 
 template <typename TIn, typename TQ, int ST>
 void run_append(const CacheAppendArgs& a, cudaStream_t stream)
 {
-    const Shape s = shape_of(a.batch.rows, a.q_heads + 2 * a.mem.heads, a.mem.head_dim);
+    const Shape s = shape_of(a.batch.rows, a.q_heads, a.mem.heads, a.mem.head_dim);
     if (a.aligned)
-        cache_append_kernel<TIn, TQ, ST, true><<<s.grid, kThreads, 0, stream>>>(a, s.tile_rows);
+        cache_append_kernel<TIn, TQ, ST, true><<<s.blocks, s.threads, 0, stream>>>(a, s.tile_rows, s.lanes);
     else
-        cache_append_kernel<TIn, TQ, ST, false><<<s.grid, kThreads, 0, stream>>>(a, s.tile_rows);
+        cache_append_kernel<TIn, TQ, ST, false><<<s.blocks, s.threads, 0, stream>>>(a, s.tile_rows, s.lanes);
 }
 
 template <typename TIn, typename TQ>
@@ -435,11 +523,11 @@ void run_append(const CacheAppendArgs& a, cudaStream_t stream)
 template <typename TOut, int ST>
 void run_read(const CacheReadArgs& a, cudaStream_t stream)
 {
-    const Shape s = shape_of(a.batch.rows, 2 * a.mem.heads, a.mem.head_dim);
+    const Shape s = shape_of(a.batch.rows, 0, a.mem.heads, a.mem.head_dim);
     if (a.aligned)
-        cache_read_kernel<TOut, ST, true><<<s.grid, kThreads, 0, stream>>>(a, s.tile_rows);
+        cache_read_kernel<TOut, ST, true><<<s.blocks, s.threads, 0, stream>>>(a, s.tile_rows, s.lanes);
     else
-        cache_read_kernel<TOut, ST, false><<<s.grid, kThreads, 0, stream>>>(a, s.tile_rows);
+        cache_read_kernel<TOut, ST, false><<<s.blocks, s.threads, 0, stream>>>(a, s.tile_rows, s.lanes);
 }
 
 template <typename TOut>
