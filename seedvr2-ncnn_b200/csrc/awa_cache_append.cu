@@ -18,7 +18,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 256;     // of cache_unpack_kernel
 constexpr int kMaxThreads = 512;  // of the others
-constexpr int kMaxTileRows = 8;
+constexpr int kMaxTileRows = 16;
 
 // Page number `index` of all that the sequences of the batch see, counted
 // sequence by sequence. Called by one full warp; the same in all lanes.
@@ -475,8 +475,10 @@ struct Shape
 
 // Heads side by side: the multiple of the cache's heads that leaves the fewest
 // threads idle over q, k and v, at 128 to 512 threads. Few rows: a block each.
-// Many: a block takes 8, so the lookup of sequence, page and coordinates is paid
-// once a tile.
+// More: a block takes several, so that the lookup of sequence, page and
+// coordinates, which its threads wait for, is paid once a tile: 4, and 16 where
+// that still leaves every SM some blocks (86074 rows: 478 us with 4, 455 with
+// 16; 1790 fp32 rows: 12.4 and 24.6).
 Shape shape_of(int rows, int q_heads, int heads, int head_dim)
 {
     Shape s;
@@ -494,7 +496,7 @@ Shape shape_of(int rows, int q_heads, int heads, int head_dim)
         }
     }
     s.threads = (s.lanes * chunks + 31) / 32 * 32;
-    s.tile_rows = rows < 148 * 8 ? 1 : kMaxTileRows;
+    s.tile_rows = rows < 148 * 8 ? 1 : rows < 148 * 64 ? 4 : kMaxTileRows;
     s.blocks = (rows + s.tile_rows - 1) / s.tile_rows;
     return s;
 }

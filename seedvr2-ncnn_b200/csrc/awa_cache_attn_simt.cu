@@ -5,6 +5,11 @@
 // sees: per block of 64 keys, S = Q K^T in registers, the running maximum m and
 // sum l of each row (base 2, scale folded into the exponent), O = O 2^(m - m')
 // + P V.
+//
+// The FMA units bound it: 4 d flops per visible pair at 128 FMAs a clock and SM.
+// Both products go through fma.f32x2, two of them per instruction, so that their
+// issue leaves room for the loads from shared memory; two blocks on an SM work
+// under each other's waits.
 #include "awa_cache_device.cuh"
 #include "awa_rows.cuh"
 
@@ -28,22 +33,43 @@ __host__ __device__ constexpr int shared_floats(int rows, int d)
     return (rows + 2 * kKeys) * (d + kPad) + rows * (kKeys + kPad);
 }
 
-__device__ __forceinline__ float dot4(float4 a, float4 b, float acc)
+using Pair = unsigned long long;  // two floats
+
+__device__ __forceinline__ Pair pair_of(float a, float b)
 {
-    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, acc))));
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
 }
 
-// T: type of the cache, q and out. A block (of a cluster of gridDim.x / tiles that share the keys) takes one
+__device__ __forceinline__ float2 floats_of(Pair p)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+
+__device__ __forceinline__ void fma2(Pair& acc, Pair a, Pair b)
+{
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+__device__ __forceinline__ void mul2(Pair& acc, Pair a)
+{
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(a));
+}
+
+// T: type of the cache, q and out. D: head_dim, 0 if only the cache knows it. A block (of a cluster of gridDim.x / tiles that share the keys) takes one
 // tile of R * 16 query rows of one key/value head. Thread (ty, tx) of 16 x 16:
 // rows ty * R + i, keys tx + 16 j, output features 4 (tx + 16 j).
-template <typename T, int R>
-__global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAttnArgs a, int cluster_size)
+template <typename T, int R, int D>
+__global__ void __launch_bounds__(kThreads, 2) cache_attention_simt_kernel(CacheAttnArgs a, int cluster_size)
 {
     constexpr int kRows = 16 * R;
     extern __shared__ float4 shared4[];
     __shared__ QueryTile tile_s;
     const CacheMemory& mem = a.mem;
-    const int d = mem.head_dim, pitch = d + kPad;
+    const int d = D ? D : mem.head_dim, pitch = d + kPad;
     float* sq = reinterpret_cast<float*>(shared4);
     float* sk = sq + kRows * pitch;
     float* sv = sk + kKeys * pitch;
@@ -90,15 +116,16 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
     const KeyBlocks blocks = key_blocks(first, last, a.sinks, kKeys);
 
     const float to_log2 = a.scale * 1.44269504088896341f;
-    float mx[R], sum[R], o[R][2][4];
+    float mx[R], sum[R];
+    Pair o[R][2][2];
 #pragma unroll
     for (int i = 0; i < R; i++)
     {
         mx[i] = -INFINITY;
         sum[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            o[i][j / 4][j % 4] = 0.f;
+        for (int j = 0; j < 4; j++)
+            o[i][j / 2][j % 2] = 0;
     }
 
     for (int n = rank; n < blocks.count; n += cluster_size)
@@ -127,28 +154,41 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
         }
         __syncthreads();
 
+        // sums over even and over odd features, added at the end
+        Pair s2[R][4];
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                s2[i][j] = 0;
+#pragma unroll 4
+        for (int f = 0; f < d; f += 4)
+        {
+            ulonglong2 qv[R], kk[4];
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                qv[i] = *reinterpret_cast<const ulonglong2*>(sq + (ty * R + i) * pitch + f);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                kk[j] = *reinterpret_cast<const ulonglong2*>(sk + (tx + 16 * j) * pitch + f);
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                {
+                    fma2(s2[i][j], qv[i].x, kk[j].x);
+                    fma2(s2[i][j], qv[i].y, kk[j].y);
+                }
+        }
         float s[R][4];
 #pragma unroll
         for (int i = 0; i < R; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                s[i][j] = 0.f;
-#pragma unroll 4
-        for (int f = 0; f < d; f += 4)
-        {
-            float4 qv[R], kk[4];
-#pragma unroll
-            for (int i = 0; i < R; i++)
-                qv[i] = *reinterpret_cast<const float4*>(sq + (ty * R + i) * pitch + f);
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                kk[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * pitch + f);
-#pragma unroll
-            for (int i = 0; i < R; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    s[i][j] = dot4(qv[i], kk[j], s[i][j]);
-        }
+            {
+                const float2 x = floats_of(s2[i][j]);
+                s[i][j] = x.x + x.y;
+            }
 #pragma unroll
         for (int i = 0; i < R; i++)
         {
@@ -178,8 +218,8 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
             }
             sum[i] = sum[i] * old + part;  // of this thread's keys; added up over tx at the end
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                o[i][j / 4][j % 4] *= old;
+            for (int j = 0; j < 4; j++)
+                mul2(o[i][j / 2][j % 2], pair_of(old, old));
         }
         __syncwarp();  // a row's probabilities come from its own half warp
 #pragma unroll 2
@@ -198,15 +238,13 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
 #pragma unroll
                 for (int u = 0; u < 4; u++)
                 {
-                    const float4 v = *reinterpret_cast<const float4*>(sv + (key + u) * pitch + f);
+                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(sv + (key + u) * pitch + f);
 #pragma unroll
                     for (int i = 0; i < R; i++)
                     {
                         const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
-                        o[i][j][0] = fmaf(w, v.x, o[i][j][0]);
-                        o[i][j][1] = fmaf(w, v.y, o[i][j][1]);
-                        o[i][j][2] = fmaf(w, v.z, o[i][j][2]);
-                        o[i][j][3] = fmaf(w, v.w, o[i][j][3]);
+                        fma2(o[i][j][0], pair_of(w, w), v.x);
+                        fma2(o[i][j][1], pair_of(w, w), v.y);
                     }
                 }
             }
@@ -234,8 +272,12 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
             for (int j = 0; j < 2; j++)
                 if (4 * (tx + 16 * j) < d)
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        store1(dst + 4 * (tx + 16 * j) + c, o[i][j][c] * inv);
+                    for (int c = 0; c < 2; c++)
+                    {
+                        const float2 x = floats_of(o[i][j][c]);
+                        store1(dst + 4 * (tx + 16 * j) + 2 * c, x.x * inv);
+                        store1(dst + 4 * (tx + 16 * j) + 2 * c + 1, x.y * inv);
+                    }
         }
         return;
     }
@@ -253,8 +295,8 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
 #pragma unroll
         for (int j = 0; j < 2; j++)
             if (4 * (tx + 16 * j) < d)
-                *reinterpret_cast<float4*>(part_o + r * pitch + 4 * (tx + 16 * j)) =
-                    make_float4(o[i][j][0], o[i][j][1], o[i][j][2], o[i][j][3]);
+                *reinterpret_cast<ulonglong2*>(part_o + r * pitch + 4 * (tx + 16 * j)) =
+                    make_ulonglong2(o[i][j][0], o[i][j][1]);
         if (tx == 0)
             part_ml[r] = make_float2(mx[i], sum[i]);
     }
@@ -290,24 +332,34 @@ __global__ void __launch_bounds__(kThreads) cache_attention_simt_kernel(CacheAtt
     cluster.sync();  // a block's shared memory stays until every peer has read it
 }
 
-template <typename T, int R>
+template <typename T, int R, int D>
 int run(const CacheAttnArgs& a, cudaStream_t stream)
 {
-    const int d = a.mem.head_dim;
-    const int64_t tiles = (int64_t)a.batch.rows * a.group / (16 * R) + a.batch.sequences;
-    // Blocks that share a tile's keys: enough to fill the GPU, at most 8 (the
-    // portable cluster size), each with at least two blocks of keys where the
-    // page table's width says how many there can be.
+    const int64_t rows = (int64_t)a.batch.rows * a.group;
+    const int64_t tiles = rows / (16 * R) + a.batch.sequences;
+    // Blocks that share a tile's keys, at most 8 (the portable cluster size): an
+    // SM's blocks share its FMA units, so what counts is the most that one SM
+    // gets of them, times the length of each -- plus a little for the join. Where
+    // the page table's width says so, each has at least two blocks of keys.
     const int64_t most = (((int64_t)a.batch.table_width << a.mem.page_shift) + kKeys - 1) / kKeys;
+    const int64_t full = (rows + 16 * R - 1) / (16 * R) + a.batch.sequences / 2;
     int cluster = 1;
-    while (cluster < 8 && tiles * a.mem.heads * cluster < 2 * 148 && most >= 4 * cluster)
-        cluster *= 2;
+    double best = 1e30;
+    for (int c = 1; c <= 8 && (c == 1 || most >= 2 * c); c *= 2)
+    {
+        const double cost = (double)((full * a.mem.heads * c + 147) / 148) / c + 0.02 * c;
+        if (cost < best)
+        {
+            best = cost;
+            cluster = c;
+        }
+    }
     if (tiles * cluster > 0x7fffffff)
         return (int)cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(tiles * cluster), (unsigned)a.mem.heads);
     config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = shared_floats(16 * R, d) * sizeof(float);
+    config.dynamicSmemBytes = shared_floats(16 * R, a.mem.head_dim) * sizeof(float);
     config.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -316,7 +368,21 @@ int run(const CacheAttnArgs& a, cudaStream_t stream)
     attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&config, cache_attention_simt_kernel<T, R>, a, cluster);
+    return (int)cudaLaunchKernelEx(&config, cache_attention_simt_kernel<T, R, D>, a, cluster);
+}
+
+template <typename T, int R>
+int run(const CacheAttnArgs& a, cudaStream_t stream)
+{
+    // bf16 caches of 64 and 128 features have kernels on the tensor cores
+    if constexpr (sizeof(T) == 4)
+    {
+        if (a.mem.head_dim == 128)
+            return run<T, R, 128>(a, stream);
+        if (a.mem.head_dim == 64)
+            return run<T, R, 64>(a, stream);
+    }
+    return run<T, R, 0>(a, stream);
 }
 
 template <typename T>
@@ -337,20 +403,25 @@ int launch_cache_attention_simt(const CacheAttnArgs& a, int max_rows, cudaStream
 
 int prepare_cache_attention_simt()
 {
-    const auto set = [](const void* kernel, int rows) {
-        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    shared_floats(rows, kMaxHeadDim) * (int)sizeof(float));
-    };
-    const void* kernels[2][2] = {
-        {(const void*)cache_attention_simt_kernel<float, 1>, (const void*)cache_attention_simt_kernel<float, 4>},
-        {(const void*)cache_attention_simt_kernel<bf16, 1>, (const void*)cache_attention_simt_kernel<bf16, 4>}};
-    for (auto& pair : kernels)
-        for (int r = 0; r < 2; r++)
-        {
-            const cudaError_t err = set(pair[r], r ? 64 : 16);
-            if (err != cudaSuccess)
-                return (int)err;
-        }
+    const struct
+    {
+        const void* kernel;
+        int rows;
+    } kernels[] = {{(const void*)cache_attention_simt_kernel<float, 1, 0>, 16},
+                   {(const void*)cache_attention_simt_kernel<float, 4, 0>, 64},
+                   {(const void*)cache_attention_simt_kernel<float, 1, 64>, 16},
+                   {(const void*)cache_attention_simt_kernel<float, 4, 64>, 64},
+                   {(const void*)cache_attention_simt_kernel<float, 1, 128>, 16},
+                   {(const void*)cache_attention_simt_kernel<float, 4, 128>, 64},
+                   {(const void*)cache_attention_simt_kernel<bf16, 1, 0>, 16},
+                   {(const void*)cache_attention_simt_kernel<bf16, 4, 0>, 64}};
+    for (const auto& k : kernels)
+    {
+        const cudaError_t err = cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     shared_floats(k.rows, kMaxHeadDim) * (int)sizeof(float));
+        if (err != cudaSuccess)
+            return (int)err;
+    }
     return 0;
 }
 
