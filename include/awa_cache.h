@@ -151,7 +151,7 @@ int awa_cache_read(const awa_cache* cache, const awa_cache_batch* batch, int out
  * statistics). 16-byte aligned rows. scale: > 0. sinks and window: 0 or more,
  * frame_tokens: 1 or more. Values in the cache that some row of the batch sees
  * have to be finite, of an AWA_INT4 cache below 2^32. workspace: awa_cache_attention_workspace_bytes() bytes,
- * 16-byte aligned (NULL if that is 0), used by this call until its work is
+ * 256-byte aligned (NULL if that is 0), used by this call until its work is
  * done: calls that may overlap, two captured graphs among them, need one each.
  * It holds the parts of rows that several blocks work on (few rows, long
  * caches) and, for many rows over an AWA_INT4 cache, the visible pages as bf16

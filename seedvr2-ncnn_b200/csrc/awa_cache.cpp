@@ -435,8 +435,8 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
     if (!aligned(q, q_token_stride * e, 16) || !aligned(out, out_token_stride * e, 16))
         return fail(AWA_ERR_INVALID, "awa_cache_attention: q and out need 16-byte aligned rows");
     const size_t need = awa_cache_attention_workspace_bytes(cache, batch, q_heads, sinks, window, frame_tokens);
-    if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)))
-        return fail(AWA_ERR_INVALID, "awa_cache_attention: 16-byte aligned workspace of %zu bytes needed, %zu given",
+    if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
+        return fail(AWA_ERR_INVALID, "awa_cache_attention: 256-byte aligned workspace of %zu bytes needed, %zu given",
                     need, workspace_bytes);
     rc = check_device(kWhat, cache);
     if (rc)

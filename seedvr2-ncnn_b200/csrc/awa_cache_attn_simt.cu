@@ -339,15 +339,16 @@ int run(const CacheAttnArgs& a, cudaStream_t stream)
     const int64_t tiles = rows / (16 * R) + a.batch.sequences;
     // Blocks that share a tile's keys, at most 8 (the portable cluster size): an
     // SM's blocks share its FMA units, so what counts is the most that one SM
-    // gets of them, times the length of each -- plus a little for the join. Where
-    // the page table's width says so, each has at least two blocks of keys.
+    // gets of them, times the length of each -- plus what a block pays for its
+    // start and the join, about 4 blocks of keys (160 tiles of 14: 291, 236, 244
+    // and 313 us with 1, 2, 4 and 8).
     const int64_t most = (((int64_t)a.batch.table_width << a.mem.page_shift) + kKeys - 1) / kKeys;
     const int64_t full = (rows + 16 * R - 1) / (16 * R) + a.batch.sequences / 2;
     int cluster = 1;
     double best = 1e30;
-    for (int c = 1; c <= 8 && (c == 1 || most >= 2 * c); c *= 2)
+    for (int c = 1; c <= 8; c *= 2)
     {
-        const double cost = (double)((full * a.mem.heads * c + 147) / 148) / c + 0.02 * c;
+        const double cost = (double)((full * a.mem.heads * c + 147) / 148) / c + 4.0 * c / (double)(most > 0 ? most : 1);
         if (cost < best)
         {
             best = cost;
