@@ -565,7 +565,6 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
     // The exponentials are taken from `top`, the largest score when it was last
     // looked for: until one exceeds it by 8 (log2) they stay below 2^8, and the
     // lanes need not meet.
-    const float slack = 8.f / to_log2;
     float local[NQ][2];
     bool grew = false;
 #pragma unroll
@@ -577,7 +576,7 @@ __device__ __forceinline__ void consume(const CacheAttnArgs& a, const Piece& p, 
 #pragma unroll
             for (int b = 1; b < kBlocks; b++)
                 local[x][c] = fmaxf(local[x][c], fmaxf(s[b][x][c], s[b][x][c + 2]));
-            grew |= local[x][c] > w.top[x][c] + slack;
+            grew |= (local[x][c] - w.top[x][c]) * to_log2 > 8.f;  // from -inf: always; -inf - -inf: never
         }
     if (__any_sync(0xffffffffu, grew))
 #pragma unroll

@@ -219,7 +219,7 @@ def test_max_rows_chooses_only_the_kernel(rows, told, storage):
 
 @pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
 @pytest.mark.parametrize("rows", [1, 150])
-@pytest.mark.parametrize("scale", [3.0, 1e-4])
+@pytest.mark.parametrize("scale", [3.0, 1e-4, 1e-38])
 def test_peaked_and_flat_softmax(rows, scale, storage):
     # scores up to a few hundred, and all but equal
     c = Batch([rows], [900], 32, 2, 128, storage, seed=9)
@@ -355,6 +355,34 @@ def test_captured_step_serves_later_steps(width, storage):
         want = step()
         assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want)
         assert not want.isnan().any()
+    awa_b200.device_status()
+
+
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+def test_captured_prompt(storage):
+    """Many rows in a graph, replayed with other lengths and page numbers."""
+    dtype = torch.float32 if storage == "f32" else torch.bfloat16
+    c = Batch([150, 90], [200, 300], 16, 2, 128, storage, seed=18)
+    cache, batch = c.handles(awa_b200)
+    q = c.new_rows(4, dtype)
+
+    def step():
+        return cache.attention(batch, q, sinks=4, window=60)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for starts, past in (([0, 150, 240], [200, 300]), ([0, 3, 240], [340, 100]), ([0, 240, 240], [90, 0])):
+        c.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+        c.past_t.copy_(torch.tensor(past, dtype=torch.int32))
+        q.copy_(torch.randn(q.shape, generator=c.generator).to(dtype))
+        for t in ((c.k, c.v) if storage != "int4" else c.params):
+            t.nan_to_num_(0.25)
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, step()) and not got.isnan().any()
     awa_b200.device_status()
 
 
