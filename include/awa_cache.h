@@ -147,15 +147,16 @@ int awa_cache_read(const awa_cache* cache, const awa_cache_batch* batch, int out
  *   need not be there: their page_table entries are not read.
  * q and out: rows x q_heads x head_dim (dense within a row) of AWA_F32 for an
  * AWA_F32 cache (fp32 FFMA, fp32 accumulation, no TF32), else of AWA_BF16
- * (bf16 operands on the tensor cores, fp32 accumulation and softmax
+ * (16-bit operands on the tensor cores, fp32 accumulation and softmax
  * statistics). 16-byte aligned rows. scale: > 0. sinks and window: 0 or more,
  * frame_tokens: 1 or more. Values in the cache that some row of the batch sees
- * have to be finite, of an AWA_INT4 cache below 2^32. workspace: awa_cache_attention_workspace_bytes() bytes,
- * 256-byte aligned (NULL if that is 0), used by this call until its work is
- * done: calls that may overlap, two captured graphs among them, need one each.
+ * have to be finite; with an AWA_INT4 cache they and q are of fp16's range,
+ * below 65504 (its products run on fp16 operands where there are many rows).
+ * workspace: awa_cache_attention_workspace_bytes() bytes, 256-byte aligned
+ * (NULL if that is 0), used by this call until its work is done: calls that may overlap, two captured graphs among them, need one each.
  * It holds the parts of rows that several blocks work on (few rows, long
- * caches) and, for many rows over an AWA_INT4 cache, the visible pages as bf16
- * (rounded once); other calls need none. */
+ * caches) and, for many rows over an AWA_INT4 cache, q and the visible pages
+ * as fp16 (rounded once); other calls need none. */
 size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int sinks,
                                            int window, int frame_tokens);
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,

@@ -333,7 +333,7 @@ enum Kernel
 {
     kStep,        // few rows per head: bf16 and 4 bits
     kTile,        // many rows: bf16
-    kUnpackTile,  // many rows of a 4-bit cache: its visible pages become bf16 first
+    kUnpackTile,  // many rows of a 4-bit cache: its visible pages become fp16 first
     kSimt
 };
 
@@ -365,21 +365,22 @@ static int64_t most_pages(const awa::CacheMemory& mem, const awa::CacheBatch& ba
     return some < all ? some : all;
 }
 
-// The workspace of kUnpackTile ahead of the tile kernel's: keys, values, page table, each on 256 bytes.
+// The workspace of kUnpackTile ahead of the tile kernel's: keys, values, page table, queries, each on 256 bytes.
 struct Unpacked
 {
     int64_t pages;
-    size_t page_bytes, pool_bytes, table_bytes;
+    size_t page_bytes, pool_bytes, table_bytes, q_bytes;
 };
 
-static Unpacked unpacked_of(const awa::CacheMemory& mem, const awa::CacheBatch& batch, int sinks, int window,
-                            int frame_tokens)
+static Unpacked unpacked_of(const awa::CacheMemory& mem, const awa::CacheBatch& batch, int q_heads, int sinks,
+                            int window, int frame_tokens)
 {
     Unpacked u;
     u.pages = most_pages(mem, batch, sinks, window, frame_tokens);
     u.page_bytes = ((size_t)mem.heads * mem.head_dim * 2) << mem.page_shift;
     u.pool_bytes = u.pages * u.page_bytes;
     u.table_bytes = ((size_t)batch.sequences * batch.table_width * 4 + 255) / 256 * 256;
+    u.q_bytes = ((size_t)batch.rows * q_heads * mem.head_dim * 2 + 255) / 256 * 256;
     return u;
 }
 
@@ -402,8 +403,8 @@ size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cac
     const size_t parts = awa::cache_attention_tile_workspace(cache->mem.head_dim);
     if (kernel == kTile)
         return parts;
-    const Unpacked u = unpacked_of(cache->mem, b, sinks, window, frame_tokens);
-    return 2 * u.pool_bytes + u.table_bytes + parts;
+    const Unpacked u = unpacked_of(cache->mem, b, q_heads, sinks, window, frame_tokens);
+    return 2 * u.pool_bytes + u.table_bytes + u.q_bytes + parts;
 }
 
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,
@@ -459,11 +460,11 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
         err = awa::launch_cache_attention_step(a, batch->max_rows,
                                                most_seen(a.mem, *batch, sinks, window, frame_tokens), workspace, s);
         break;
-    case kTile: err = awa::launch_cache_attention_tile(a, workspace, s); break;
+    case kTile: err = awa::launch_cache_attention_tile(a, false, workspace, s); break;
     case kSimt: err = awa::launch_cache_attention_simt(a, batch->max_rows, s); break;
     case kUnpackTile:
     {
-        const Unpacked u = unpacked_of(a.mem, a.batch, sinks, window, frame_tokens);
+        const Unpacked u = unpacked_of(a.mem, a.batch, q_heads, sinks, window, frame_tokens);
         if (u.pages > 0x7fffffff)
             return fail(AWA_ERR_INVALID, "awa_cache_attention: the batch reaches too many pages");
         awa::CacheUnpackArgs unpack{};
@@ -475,8 +476,13 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
         unpack.k_out = static_cast<char*>(workspace);
         unpack.v_out = unpack.k_out + u.pool_bytes;
         unpack.table = reinterpret_cast<int*>(unpack.v_out + u.pool_bytes);
+        unpack.q_out = reinterpret_cast<char*>(unpack.table) + u.table_bytes;
+        unpack.q = q;
+        unpack.q_stride = q_token_stride;
+        unpack.q_row = (int)row;
+        unpack.pages = (int)u.pages;
         unpack.error_flag = a.error_flag;
-        err = awa::launch_cache_unpack(unpack, (int)u.pages, s);
+        err = awa::launch_cache_unpack(unpack, s);
         if (err)
             break;
         a.mem.storage = AWA_BF16;
@@ -487,7 +493,9 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
         a.mem.head_stride = (int64_t)u.page_bytes / a.mem.heads;
         a.batch.page_table = unpack.table;
         a.batch.table_stride = a.batch.table_width;
-        err = awa::launch_cache_attention_tile(a, reinterpret_cast<char*>(unpack.table) + u.table_bytes, s);
+        a.q = unpack.q_out;
+        a.q_stride = row;
+        err = awa::launch_cache_attention_tile(a, true, unpack.q_out + u.q_bytes, s);
         break;
     }
     }

@@ -8,6 +8,7 @@
 #include "awa_cache_device.cuh"
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 namespace awa
 {
@@ -411,13 +412,41 @@ __global__ void __launch_bounds__(kMaxThreads, 2) cache_read_kernel(CacheReadArg
     }
 }
 
-// One 4-bit page that some row of the batch sees -> its keys and values as
-// bf16, and its number in the workspace's page table. Blocks: x = the pages of
-// all sequences in order, y = heads.
+// 8 floats as fp16.
+__device__ __forceinline__ uint4 half8(const float (&v)[8])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One 4-bit page that some row of the batch sees -> its keys and values as fp16
+// (rounded by 2^-12, where bf16's 2^-9 of every key would show in the scores),
+// and its number in the workspace's page table. Blocks: x = the pages of all
+// sequences in order, y = heads; the blocks x behind them take the q rows.
 __global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs a)
 {
     __shared__ int which_s[2];
     const CacheMemory& mem = a.mem;
+    if ((int)blockIdx.x >= a.pages)
+    {
+        const int64_t chunks = a.q_row / 8, all = chunks * a.batch.rows;
+        const int64_t step = (int64_t)(gridDim.x - a.pages) * gridDim.y * kThreads;
+        int64_t i = ((int64_t)(blockIdx.x - a.pages) * gridDim.y + blockIdx.y) * kThreads + threadIdx.x;
+        for (; i < all; i += step)
+        {
+            const int64_t row = i / chunks;
+            float v[8];
+            load8(static_cast<const bf16*>(a.q) + row * a.q_stride + (i - row * chunks) * 8, v);
+            reinterpret_cast<uint4*>(a.q_out)[i] = half8(v);
+        }
+        return;
+    }
     if (threadIdx.x < 32)
     {
         const PageSlot at = find_page(a, blockIdx.x);
@@ -458,9 +487,9 @@ __global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs 
                 reinterpret_cast<const uint32_t*>((is_k ? mem.k_params : mem.v_params) + par) + row * groups + group);
             float v[8];
             dequantize8(codes.x, params, v);
-            store8(reinterpret_cast<bf16*>(&out[0]), v);
+            out[0] = half8(v);
             dequantize8(codes.y, params, v);
-            store8(reinterpret_cast<bf16*>(&out[1]), v);
+            out[1] = half8(v);
         }
         uint4* to = reinterpret_cast<uint4*>((is_k ? a.k_out : a.v_out) + dst + (int64_t)at * 4);
         to[0] = out[0];
@@ -562,10 +591,13 @@ int launch_cache_read(const CacheReadArgs& a, int out_dtype, cudaStream_t stream
     return (int)cudaGetLastError();
 }
 
-int launch_cache_unpack(const CacheUnpackArgs& a, int pages, cudaStream_t stream)
+int launch_cache_unpack(const CacheUnpackArgs& a, cudaStream_t stream)
 {
     ProfileScope scope("awa_cache_unpack", stream);
-    cache_unpack_kernel<<<dim3((unsigned)pages, (unsigned)a.mem.heads), kThreads, 0, stream>>>(a);
+    // 4 pieces of q a thread
+    const int64_t pieces = (int64_t)a.batch.rows * (a.q_row / 8);
+    const int64_t q_blocks = (pieces + 4 * kThreads * a.mem.heads - 1) / (4 * kThreads * a.mem.heads);
+    cache_unpack_kernel<<<dim3((unsigned)(a.pages + q_blocks), (unsigned)a.mem.heads), kThreads, 0, stream>>>(a);
     return (int)cudaGetLastError();
 }
 

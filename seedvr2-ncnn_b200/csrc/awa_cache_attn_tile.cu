@@ -40,6 +40,7 @@
 
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <mutex>
 
@@ -597,11 +598,19 @@ __device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar)
         : "memory");
 }
 
+// Instruction descriptor: bf16 operands, or fp16 (Q, K, P and V alike) for what
+// was unpacked from 4 bits.
+template <bool HALF>
+__device__ __forceinline__ uint32_t operands(int n, bool b_mn_major)
+{
+    return tc::idesc_bf16_f32(128, n, b_mn_major) & (HALF ? ~((1u << 7) | (1u << 10)) : ~0u);
+}
+
 // S[128 x 128] = Q K^T, both K-major in panels of 64 features.
-template <int D>
+template <int D, bool HALF>
 __device__ __forceinline__ void issue_qk(uint32_t leader, uint32_t tmem_s, uint32_t q_addr, uint32_t k_addr)
 {
-    const uint32_t idesc = tc::idesc_bf16_f32(128, kKeys, false);
+    const uint32_t idesc = operands<HALF>(kKeys, false);
     const uint64_t q = tc::smem_desc_sw128(q_addr, 16, 1024), k = tc::smem_desc_sw128(k_addr, 16, 1024);
 #pragma unroll
     for (int s = 0; s < D / 16; s++)
@@ -616,11 +625,11 @@ __device__ __forceinline__ void issue_qk(uint32_t leader, uint32_t tmem_s, uint3
 
 // O[128 x D] (+)= P[128 x 128] V[128 x D], P in TMEM, V MN-major: 8-key groups
 // 1024 bytes apart, panels of 64 features kPanelBytes apart. One half of the keys.
-template <int D>
+template <int D, bool HALF>
 __device__ __forceinline__ void issue_pv(uint32_t leader, uint32_t tmem_o, uint32_t tmem_p, uint32_t v_addr,
                                          uint32_t accumulate, int half)
 {
-    const uint32_t idesc = tc::idesc_bf16_f32(128, D, true);
+    const uint32_t idesc = operands<HALF>(D, true);
     const uint64_t v = tc::smem_desc_sw128(v_addr, Tile<D>::kPanelBytes, 1024);
 #pragma unroll
     for (int s = half * kKeys / 32; s < (half + 1) * kKeys / 32; s++)
@@ -634,7 +643,7 @@ __device__ __forceinline__ int uniform(int x)
     return __shfl_sync(0xffffffffu, x, 0);
 }
 
-template <int D>
+template <int D, bool HALF>
 __device__ void mma_issue(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem_any)
 {
     using T = Tile<D>;
@@ -701,7 +710,7 @@ __device__ void mma_issue(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem_any
         // scale O once the scores are in.
         if (then[x])
         {
-            issue_qk<D>(leader, tmem + kColS + 128 * x, q0 + x * T::kBytes, ring + k_stage * T::kBytes);
+            issue_qk<D, HALF>(leader, tmem + kColS + 128 * x, q0 + x * T::kBytes, ring + k_stage * T::kBytes);
             commit(leader, &sh.s_full[x]);
         }
         now[x] = then[x];
@@ -786,7 +795,7 @@ __device__ void mma_issue(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem_any
                         if (!wait(&sh.p_full[x][h], (p_phase >> x) & 1, 84))
                             return;
                         tc::fence_after_sync();
-                        issue_pv<D>(leader, tmem + kColO + 128 * x, tmem + kColS + 128 * x, v_addr, (started >> x) & 1,
+                        issue_pv<D, HALF>(leader, tmem + kColO + 128 * x, tmem + kColS + 128 * x, v_addr, (started >> x) & 1,
                                     h);
                     }
                     p_phase ^= 1u << x;
@@ -808,10 +817,10 @@ __device__ void mma_issue(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem_any
     }
 }
 
-template <int D>
+template <int D, bool HALF>
 __device__ void mma_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem)
 {
-    mma_issue<D>(a, sh, tmem);
+    mma_issue<D, HALF>(a, sh, tmem);
     commit(elect_one(), &sh.mma_done);
     __syncwarp();
     drain_bar(&sh.mma_done, 0, a.error_flag, 85);  // complete before TMEM is released
@@ -876,9 +885,18 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8])
                  : "memory");
 }
 
+template <bool HALF>
+__device__ __forceinline__ uint32_t operand_pair(float lo, float hi)
+{
+    if (!HALF)
+        return pack_bf16x2(lo, hi);
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // part_o, part_ml: the sums of unfinished jobs, [slot][tile][row] of D features
 // and (maximum, sum).
-template <int D>
+template <int D, bool HALF>
 __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem, float* part_o, float2* part_ml)
 {
     const int warp = threadIdx.x >> 5;
@@ -993,7 +1011,7 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem,
                     fma_x2(x0, x1, __uint_as_float(v[k]), __uint_as_float(v[k + 1]), scale_log2, neg_m);
                     const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
                     add_x2(sums[2 * (j & 1)], sums[2 * (j & 1) + 1], p0, p1);
-                    pk[j] = pack_bf16x2(p0, p1);  // the operand type of P V; the sums keep fp32
+                    pk[j] = operand_pair<HALF>(p0, p1);  // the operand type of P V; the sums keep fp32
                 }
                 tc::tmem_st16(t_s + 16 * c, pk);
                 if (c & 1)  // half of the keys
@@ -1069,7 +1087,7 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem,
     }
 }
 
-template <int D>
+template <int D, bool HALF>
 __global__ void __launch_bounds__(kThreads, 1)
     cache_attention_tile_kernel(const CacheAttnArgs a, const __grid_constant__ Maps maps, float* part_o,
                                 float2* part_ml, Joint* joint)
@@ -1184,13 +1202,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp < kSoftmaxWarps)
     {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        softmax_role<D>(a, sh, tmem, part_o, part_ml);
+        softmax_role<D, HALF>(a, sh, tmem, part_o, part_ml);
     }
     else
     {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kMmaWarp)
-            mma_role<D>(a, sh, tmem);
+            mma_role<D, HALF>(a, sh, tmem);
         else if (warp == kTmaWarp)
             tma_role<D>(a, maps, sh);
         else if (warp == kCleanWarp)
@@ -1309,7 +1327,7 @@ constexpr size_t workspace_bytes()
 
 static_assert(sizeof(Tile<128>) <= 232448 && sizeof(Tile<64>) <= 232448, "shared memory of a block");
 
-template <int D>
+template <int D, bool HALF>
 int run(const CacheAttnArgs& a, void* workspace, cudaStream_t stream)
 {
     Maps maps;
@@ -1326,7 +1344,7 @@ int run(const CacheAttnArgs& a, void* workspace, cudaStream_t stream)
     float* part_o = static_cast<float*>(workspace);
     float2* part_ml = reinterpret_cast<float2*>(part_o + (size_t)2 * kBlocks * 2 * kRows * D);
     Joint* joint = reinterpret_cast<Joint*>(part_ml + (size_t)2 * kBlocks * 2 * kRows);
-    cache_attention_tile_kernel<D>
+    cache_attention_tile_kernel<D, HALF>
         <<<kBlocks, kThreads, sizeof(Tile<D>), stream>>>(a, maps, part_o, part_ml, joint);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess)
@@ -1345,10 +1363,10 @@ int run(const CacheAttnArgs& a, void* workspace, cudaStream_t stream)
                                    (const float2*)part_ml, (const Joint*)joint);
 }
 
-template <int D>
+template <int D, bool HALF>
 cudaError_t prepare()
 {
-    return cudaFuncSetAttribute(cache_attention_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(cache_attention_tile_kernel<D, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 (int)sizeof(Tile<D>));
 }
 
@@ -1364,16 +1382,23 @@ int cache_attention_tile_sequences()
     return kMostSequences;
 }
 
-int launch_cache_attention_tile(const CacheAttnArgs& a, void* workspace, cudaStream_t stream)
+int launch_cache_attention_tile(const CacheAttnArgs& a, bool half, void* workspace, cudaStream_t stream)
 {
     ProfileScope scope("awa_cache_attention_tile", stream);
-    return a.mem.head_dim == 64 ? run<64>(a, workspace, stream) : run<128>(a, workspace, stream);
+    if (a.mem.head_dim == 64)
+        return half ? run<64, true>(a, workspace, stream) : run<64, false>(a, workspace, stream);
+    return half ? run<128, true>(a, workspace, stream) : run<128, false>(a, workspace, stream);
 }
 
 int prepare_cache_attention_tile()
 {
-    const cudaError_t err = prepare<64>();
-    return (int)(err != cudaSuccess ? err : prepare<128>());
+    for (cudaError_t (*set)() : {prepare<64, false>, prepare<64, true>, prepare<128, false>, prepare<128, true>})
+    {
+        const cudaError_t err = set();
+        if (err != cudaSuccess)
+            return (int)err;
+    }
+    return 0;
 }
 
 }  // namespace awa

@@ -66,15 +66,20 @@ struct CacheReadArgs
     int* error_flag;
 };
 
-// 4-bit pages that a batch sees -> dense bf16 pages [page][head][slot][head_dim]
-// and a page table [sequences][table_width] of theirs.
+// 4-bit pages that a batch sees -> dense fp16 pages [page][head][slot][head_dim]
+// and a page table [sequences][table_width] of theirs; the batch's q rows, bf16
+// -> dense fp16.
 struct CacheUnpackArgs
 {
     CacheMemory mem;
     CacheBatch batch;
     int sinks, window, frame_tokens;
-    char *k_out, *v_out;
+    char *k_out, *v_out, *q_out;
     int* table;
+    const void* q;
+    int64_t q_stride;
+    int q_row;  // elements of a row
+    int pages;  // as many as the batch can see, at most
     int* error_flag;
 };
 
@@ -94,8 +99,7 @@ struct CacheAttnArgs
 
 int launch_cache_append(const CacheAppendArgs& args, int in_dtype, int q_out_dtype, cudaStream_t stream);
 int launch_cache_read(const CacheReadArgs& args, int out_dtype, cudaStream_t stream);
-// pages: as many as the batch can see, at most.
-int launch_cache_unpack(const CacheUnpackArgs& args, int pages, cudaStream_t stream);
+int launch_cache_unpack(const CacheUnpackArgs& args, cudaStream_t stream);
 // fp32 and bf16 caches of any head_dim, fp32 arithmetic.
 int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStream_t stream);
 // bf16 and 4-bit caches with head_dim 64 or 128, for few rows per sequence;
@@ -108,7 +112,8 @@ int launch_cache_attention_step(const CacheAttnArgs& args, int max_rows, int64_t
 // head, for many rows per sequence.
 size_t cache_attention_tile_workspace(int head_dim);
 int cache_attention_tile_sequences();  // the most it takes
-int launch_cache_attention_tile(const CacheAttnArgs& args, void* workspace, cudaStream_t stream);
+// half: q, k and v hold fp16 (what launch_cache_unpack writes), out bf16 as ever.
+int launch_cache_attention_tile(const CacheAttnArgs& args, bool half, void* workspace, cudaStream_t stream);
 // cudaFuncSetAttribute calls of the kernels, once per handle (not allowed to
 // fail later, inside a capture).
 int prepare_cache_attention_simt();
