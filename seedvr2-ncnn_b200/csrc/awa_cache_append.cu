@@ -4,7 +4,9 @@
 // Per row and head: (x0, x1) -> (x0 c - x1 s, x1 c + x0 s) for the rotated
 // pairs of q and k, one rounding to the storage type (or to 4-bit codes with a
 // scale and a minimum per 64 features). Nothing is read or written twice, so
-// memory bounds it: bytes = rows * (q + k + v in, q + k + v out).
+// memory bounds it: bytes = rows * (q + k + v in, q + k + v out). Measured (B200):
+// 86074 rows of 20 heads of 128 in bf16, 2.64 GB, 466 us (5.7 TB/s, 0.87 of the
+// measured copy rate); 8 rows 3.9 us.
 #include "awa_cache_device.cuh"
 
 #include <cuda_bf16.h>

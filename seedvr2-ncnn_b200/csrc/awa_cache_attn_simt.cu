@@ -9,7 +9,9 @@
 // The FMA units bound it: 4 d flops per visible pair at 128 FMAs a clock and SM.
 // Both products go through fma.f32x2, two of them per instruction, so that their
 // issue leaves room for the loads from shared memory; two blocks on an SM work
-// under each other's waits.
+// under each other's waits. Measured (B200): 512 rows of 20 heads over 1594 keys
+// 236 us, 18 TFLOP/s, a quarter of the FMA rate: a tile's 14 blocks of keys are
+// few beside its start, its loads and the uneven last round of blocks.
 #include "awa_cache_device.cuh"
 #include "awa_rows.cuh"
 

@@ -24,6 +24,12 @@
 //   sum p v = sum p' c + sum p' z,  p' = bf16(p scale),
 // the sums in fp32, the last one with the same rounded p', so that the one
 // rounding acts on p as it does for a bf16 cache.
+//
+// Measured (B200): 64 streams of 500 to 32000 rows, window 8192, 32 / 8 heads:
+// 194 us, 6.0 TB/s, 0.92 of the measured copy rate. The same in 4 bits, 32
+// streams up to 32700 rows: 138 us, 4.1 TB/s, 0.63: there the instructions that
+// turn codes into operands (350 a 16 keys and warp) bound it, not memory. One
+// stream of 700 rows: 8.4 us.
 #include "awa_cache_device.cuh"
 #include "awa_rows.cuh"
 
