@@ -174,6 +174,8 @@ int create(const awa_cache_params* params, awa_cache** out, bool on_device)
         if (err == cudaSuccess)
             err = static_cast<cudaError_t>(awa::prepare_cache_attention_simt());
         if (err == cudaSuccess)
+            err = static_cast<cudaError_t>(awa::prepare_cache_attention_f32());
+        if (err == cudaSuccess)
             err = static_cast<cudaError_t>(awa::prepare_cache_attention_step());
         if (err == cudaSuccess)
             err = static_cast<cudaError_t>(awa::prepare_cache_attention_tile());
@@ -334,7 +336,8 @@ enum Kernel
     kStep,        // few rows per head: bf16 and 4 bits
     kTile,        // many rows: bf16
     kUnpackTile,  // many rows of a 4-bit cache: its visible pages become fp16 first
-    kSimt
+    kF32,         // many rows: fp32
+    kSimt         // few rows: fp32; other head sizes
 };
 
 // Up to 32 (row, head) pairs per key/value head and sequence the step kernel
@@ -342,8 +345,11 @@ enum Kernel
 // tile kernel always computes 128 of them.
 static Kernel kernel_of(const awa::CacheMemory& mem, const awa_cache_batch& batch, int group)
 {
-    if (mem.storage == AWA_F32 || (mem.head_dim != 64 && mem.head_dim != 128))
+    if (mem.head_dim != 64 && mem.head_dim != 128)
         return kSimt;
+    // 17 (row, head) pairs are more than one FMA tile of 16 holds
+    if (mem.storage == AWA_F32)
+        return (int64_t)batch.max_rows * group <= 16 ? kSimt : kF32;
     if ((int64_t)batch.max_rows * group <= 32 || group > 128 ||
         batch.sequences > awa::cache_attention_tile_sequences())
         return kStep;
@@ -398,7 +404,7 @@ size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cac
     if (kernel == kStep)
         return awa::cache_attention_step_workspace(cache->mem, group, batch->max_rows,
                                                    most_seen(cache->mem, *batch, sinks, window, frame_tokens));
-    if (kernel == kSimt)
+    if (kernel == kSimt || kernel == kF32)
         return 0;
     const size_t parts = awa::cache_attention_tile_workspace(cache->mem.head_dim);
     if (kernel == kTile)
@@ -462,6 +468,7 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
         break;
     case kTile: err = awa::launch_cache_attention_tile(a, false, workspace, s); break;
     case kSimt: err = awa::launch_cache_attention_simt(a, batch->max_rows, s); break;
+    case kF32: err = awa::launch_cache_attention_f32(a, s); break;
     case kUnpackTile:
     {
         const Unpacked u = unpacked_of(a.mem, a.batch, q_heads, sinks, window, frame_tokens);

@@ -1,5 +1,6 @@
 // awa_cache_attn_simt.cu -- attention over the paged key/value cache in fp32
-// arithmetic, for fp32 caches and for head sizes without a tensor-core kernel.
+// arithmetic, for few rows of fp32 caches and for head sizes without a
+// tensor-core kernel.
 //
 // out = softmax(scale q K^T) V in one pass over the keys a tile of query rows
 // sees: per block of 64 keys, S = Q K^T in registers, the running maximum m and
@@ -9,13 +10,13 @@
 // The FMA units bound it: 4 d flops per visible pair at 128 FMAs a clock and SM.
 // Both products go through fma.f32x2, two of them per instruction, so that their
 // issue leaves room for the loads from shared memory; two blocks on an SM work
-// under each other's waits. Measured (B200): 512 rows of 20 heads over 1594 keys
-// 236 us, 18 TFLOP/s, a quarter of the FMA rate: a tile's 14 blocks of keys are
-// few beside its start, its loads and the uneven last round of blocks.
-#include "awa_cache_device.cuh"
-#include "awa_rows.cuh"
+// under each other's waits. Measured (B200), with 128 features known when
+// compiling: 512 rows of 20 heads over 1594 keys 236 us, 18 TFLOP/s, a quarter of
+// the FMA rate: a tile's 14 blocks of keys are few beside its start, its loads and
+// the uneven last round of blocks. With 64 and 128 features such calls go to the
+// tensor cores (141 us).
+#include "awa_cache_join.cuh"
 
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 namespace awa
@@ -23,7 +24,6 @@ namespace awa
 namespace
 {
 
-namespace cg = cooperative_groups;
 using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 256;
@@ -284,9 +284,6 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_simt_kernel(Cache
         return;
     }
 
-    // The cluster's parts meet in shared memory: O, m and l of every block,
-    // joined in the order of the ranks, each block taking a share of the rows.
-    cg::cluster_group cluster = cg::this_cluster();
     __syncthreads();
     float* part_o = sq;                // [kRows][pitch]
     float2* part_ml = reinterpret_cast<float2*>(sk);
@@ -302,36 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_simt_kernel(Cache
         if (tx == 0)
             part_ml[r] = make_float2(mx[i], sum[i]);
     }
-    cluster.sync();
-    for (int i = rank * kThreads + threadIdx.x; i < t.count * (d / 4); i += cluster_size * kThreads)
-    {
-        const int r = i / (d / 4), f = (i - r * (d / 4)) * 4;
-        float top = -INFINITY;
-        for (int c = 0; c < cluster_size; c++)
-            top = fmaxf(top, cluster.map_shared_rank(part_ml, c)[r].x);
-        const float base = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = 0; c < cluster_size; c++)
-        {
-            const float2 ml = cluster.map_shared_rank(part_ml, c)[r];
-            const float w = fast_exp2(ml.x - base);
-            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part_o, c) + r * pitch + f);
-            total = fmaf(ml.y, w, total);
-            acc.x = fmaf(x.x, w, acc.x);
-            acc.y = fmaf(x.y, w, acc.y);
-            acc.z = fmaf(x.z, w, acc.z);
-            acc.w = fmaf(x.w, w, acc.w);
-        }
-        const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-        const int m = t.m0 + r;
-        T* dst = out + (int64_t)(t.row0 + m / a.group) * a.out_stride + (int64_t)(kv * a.group + m % a.group) * d + f;
-        store1(dst, acc.x * inv);
-        store1(dst + 1, acc.y * inv);
-        store1(dst + 2, acc.z * inv);
-        store1(dst + 3, acc.w * inv);
-    }
-    cluster.sync();  // a block's shared memory stays until every peer has read it
+    join_cluster<T, kThreads>(a, t, kv, d, rank, cluster_size, part_o, pitch, part_ml);
 }
 
 template <typename T, int R, int D>
@@ -339,24 +307,9 @@ int run(const CacheAttnArgs& a, cudaStream_t stream)
 {
     const int64_t rows = (int64_t)a.batch.rows * a.group;
     const int64_t tiles = rows / (16 * R) + a.batch.sequences;
-    // Blocks that share a tile's keys, at most 8 (the portable cluster size): an
-    // SM's blocks share its FMA units, so what counts is the most that one SM
-    // gets of them, times the length of each -- plus what a block pays for its
-    // start and the join, about 4 blocks of keys (160 tiles of 14: 291, 236, 244
-    // and 313 us with 1, 2, 4 and 8).
-    const int64_t most = (((int64_t)a.batch.table_width << a.mem.page_shift) + kKeys - 1) / kKeys;
-    const int64_t full = (rows + 16 * R - 1) / (16 * R) + a.batch.sequences / 2;
-    int cluster = 1;
-    double best = 1e30;
-    for (int c = 1; c <= 8; c *= 2)
-    {
-        const double cost = (double)((full * a.mem.heads * c + 147) / 148) / c + 4.0 * c / (double)(most > 0 ? most : 1);
-        if (cost < best)
-        {
-            best = cost;
-            cluster = c;
-        }
-    }
+    // a start and a join cost about 4 blocks of keys (160 tiles of 14: 291, 236, 244
+    // and 313 us with 1, 2, 4 and 8 blocks a tile)
+    const int cluster = cluster_of(a, rows, 16 * R, kKeys, 4.0);
     if (tiles * cluster > 0x7fffffff)
         return (int)cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t config = {};
@@ -377,8 +330,8 @@ int run(const CacheAttnArgs& a, cudaStream_t stream)
 template <typename T, int R>
 int run(const CacheAttnArgs& a, cudaStream_t stream)
 {
-    // bf16 caches of 64 and 128 features have kernels on the tensor cores
-    if constexpr (sizeof(T) == 4)
+    // the other sizes and types with 64 and 128 features have kernels of their own
+    if constexpr (sizeof(T) == 4 && R == 1)
     {
         if (a.mem.head_dim == 128)
             return run<T, R, 128>(a, stream);
@@ -413,9 +366,7 @@ int prepare_cache_attention_simt()
     } kernels[] = {{(const void*)cache_attention_simt_kernel<float, 1, 0>, 16},
                    {(const void*)cache_attention_simt_kernel<float, 4, 0>, 64},
                    {(const void*)cache_attention_simt_kernel<float, 1, 64>, 16},
-                   {(const void*)cache_attention_simt_kernel<float, 4, 64>, 64},
                    {(const void*)cache_attention_simt_kernel<float, 1, 128>, 16},
-                   {(const void*)cache_attention_simt_kernel<float, 4, 128>, 64},
                    {(const void*)cache_attention_simt_kernel<bf16, 1, 0>, 16},
                    {(const void*)cache_attention_simt_kernel<bf16, 4, 0>, 64}};
     for (const auto& k : kernels)

@@ -31,6 +31,7 @@
 // turn codes into operands (350 a 16 keys and warp) bound it, not memory. One
 // stream of 700 rows: 8.4 us.
 #include "awa_cache_device.cuh"
+#include "awa_mma.cuh"
 #include "awa_rows.cuh"
 
 #include <cooperative_groups.h>
@@ -71,54 +72,12 @@ struct Step
     }
 };
 
-__device__ __forceinline__ uint32_t shared_address(const void* p)
-{
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// Copies BYTES (4, 8 or 16); none of them is read, and zeros written, if !real.
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool real)
-{
-    const int n = real ? BYTES : 0;
-    if (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES)
-                     : "memory");
-}
-
-__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4])
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4])
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-
 // 8x8 transpose of one b16 matrix held across the warp.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Codes j and j + 4 of a word as the bits of two bf16 numbers: c 2^-133, for odd j 16 c 2^-133.

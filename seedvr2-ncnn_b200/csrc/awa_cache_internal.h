@@ -102,6 +102,8 @@ int launch_cache_read(const CacheReadArgs& args, int out_dtype, cudaStream_t str
 int launch_cache_unpack(const CacheUnpackArgs& args, cudaStream_t stream);
 // fp32 and bf16 caches of any head_dim, fp32 arithmetic.
 int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStream_t stream);
+// fp32 caches with head_dim 64 or 128, for many rows per sequence.
+int launch_cache_attention_f32(const CacheAttnArgs& args, cudaStream_t stream);
 // bf16 and 4-bit caches with head_dim 64 or 128, for few rows per sequence;
 // most_keys: no row sees more. The workspace holds the parts of tiles that
 // several blocks work on (0 bytes for short caches).
@@ -117,6 +119,7 @@ int launch_cache_attention_tile(const CacheAttnArgs& args, bool half, void* work
 // cudaFuncSetAttribute calls of the kernels, once per handle (not allowed to
 // fail later, inside a capture).
 int prepare_cache_attention_simt();
+int prepare_cache_attention_f32();
 int prepare_cache_attention_step();
 int prepare_cache_attention_tile();
 

@@ -427,3 +427,20 @@ def test_positions_past_four_gigabytes(storage):
     want, tol = attention(c, q, 0, 0, 1, d ** -0.5)
     assert ((out.double() - want).abs() <= tol).all()
     assert ((last.double() - want[-1:]).abs() <= tol[-1:]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 20, 150])
+def test_f32_values_of_a_single_key_come_back_exactly(rows, d):
+    """A row that sees one key gets p = 1: its value, bit for bit, up to the largest floats and over 160 binades."""
+    c = Batch([rows], [40], 16, 2, d, "f32", seed=5)
+    cache, batch = c.handles(awa_b200)
+    q = c.new_rows(2, torch.float32)
+    page, slot = c.slots(0, torch.arange(40, 40 + rows))
+    v = c.cached(0, "v")[40:].float()
+    v *= torch.exp2(torch.arange(rows * d * 2, device=v.device).reshape(rows, 2, d) % 161 - 80.0)
+    v[0, 0, 0], v[-1, 1, 1] = torch.finfo(torch.float32).max, torch.finfo(torch.float32).min
+    c.v[page, :, slot] = v
+    out = cache.attention(batch, q, window=1)
+    awa_b200.device_status()
+    assert torch.equal(out, v)
