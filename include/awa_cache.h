@@ -146,7 +146,7 @@ int awa_cache_read(const awa_cache* cache, const awa_cache_batch* batch, int out
  *   A row that sees nothing gets zeros. Pages that no row of the batch sees
  *   need not be there: their page_table entries are not read.
  * q and out: rows x q_heads x head_dim (dense within a row) of AWA_F32 for an
- * AWA_F32 cache (fp32 FFMA, fp32 accumulation, no TF32), else of AWA_BF16
+ * AWA_F32 cache (to fp32 accuracy: FFMA or six bf16 products, fp32 sums), else of AWA_BF16
  * (16-bit operands on the tensor cores, fp32 accumulation and softmax
  * statistics). 16-byte aligned rows. scale: > 0. sinks and window: 0 or more,
  * frame_tokens: 1 or more. Values in the cache that some row of the batch sees
