@@ -124,10 +124,13 @@ class CacheBatch:
         if (row_starts.stride(0) != 1 or (past.shape[0] > 1 and past.stride(0) != 1) or
                 (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
             raise ValueError("row_starts, past and the rows of page_table must be dense")
+        if past.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
+            raise ValueError("the rows of page_table must not overlap (an expanded table: .contiguous())")
         if not row_starts.device == past.device == page_table.device:
             raise ValueError("row_starts, past and page_table must be on one device")
         self.row_starts, self.past, self.page_table = row_starts, past, page_table
         self.rows, self.device = int(rows), past.device
+        # a single row's stride is never used, but has to hold a row
         width = page_table.shape[1]
         self.c = _CacheBatch(past.shape[0], self.rows, int(max_rows), row_starts.data_ptr(), past.data_ptr(),
                              page_table.data_ptr(), width, max(page_table.stride(0), width))
