@@ -102,9 +102,9 @@ typedef struct
     const int* coords;  /* [rows][axes]; NULL: every axis takes the row's position in its sequence */
 } awa_cache_rope;
 
-/* Checks the parameters and builds the handle on the CURRENT device (tensor
- * maps of the memory, the status flag, the kernels' attributes): make it before
- * a stream capture begins. Holds no device memory of its own. */
+/* Checks the parameters and builds the handle on the CURRENT device (the status
+ * flag, the kernels' attributes), where the memory has to lie: make it before a
+ * stream capture begins. Holds no device memory of its own. */
 int awa_cache_create(const awa_cache_params* params, awa_cache** out);
 /* The checks of awa_cache_create without a device: for checking arguments on
  * machines without a GPU. Every call that would enqueue work rejects such a

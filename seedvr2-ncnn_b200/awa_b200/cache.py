@@ -142,7 +142,8 @@ class KvCache:
     head_dim] bf16 or fp32, or uint8 [..., head_dim / 2] with k_params, v_params
     bf16 [pages, heads, page_tokens, head_dim / 64, 2] (scale, minimum) for 4
     bits. k and v may be views with other page and head strides (the same for
-    both)."""
+    both). The handle belongs to their device, which has to be current in the
+    calls. host_only: a handle that only checks arguments (awa_cache_create_host)."""
 
     def __init__(self, k, v, k_params=None, v_params=None, host_only: bool = False):
         torch = _torch()
@@ -156,6 +157,8 @@ class KvCache:
             raise ValueError("k and v are [pages, heads, page_tokens, head_dim] with equal strides and dtype")
         if any(t.device != k.device for t in tensors):
             raise ValueError("the cache's tensors must be on one device")
+        if not host_only and k.device.type != "cuda":
+            raise ValueError("the cache's tensors must be CUDA tensors")
         pages, heads, page_tokens, row = k.shape
         self.head_dim = row * 2 if four else row
         if k.stride(3) != 1 or k.stride(2) != row:
@@ -171,8 +174,11 @@ class KvCache:
             params.k_params, params.v_params = k_params.data_ptr(), v_params.data_ptr()
             params.params_page_stride, params.params_head_stride = k_params.stride(0), k_params.stride(1)
         handle = ctypes.c_void_p()
-        create = lib.awa_cache_create_host if host_only else lib.awa_cache_create
-        _check(create(ctypes.byref(params), ctypes.byref(handle)))
+        if host_only:
+            _check(lib.awa_cache_create_host(ctypes.byref(params), ctypes.byref(handle)))
+        else:
+            with torch.cuda.device(k.device):  # the handle belongs to the current device
+                _check(lib.awa_cache_create(ctypes.byref(params), ctypes.byref(handle)))
         self._handle = handle.value
         self.k, self.v, self.k_params, self.v_params = k, v, k_params, v_params
         self.heads, self.storage, self.device = heads, storage, k.device

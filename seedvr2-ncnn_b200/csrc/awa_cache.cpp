@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <new>
 
 #include <cuda_runtime.h>
@@ -137,6 +138,30 @@ int check_device(const char* what, const awa_cache* cache)
     return AWA_OK;
 }
 
+// The memory of a cache lies where a kernel on `device` reaches it.
+int check_memory(const awa_cache_params& p, int device)
+{
+    const bool four = p.storage == AWA_INT4;
+    for (const void* memory : {p.k, p.v, four ? p.k_params : nullptr, four ? p.v_params : nullptr})
+    {
+        if (!memory)
+            continue;
+        cudaPointerAttributes at{};
+        const cudaError_t err = cudaPointerGetAttributes(&at, memory);
+        if (err != cudaSuccess)
+        {
+            cudaGetLastError();  // not the caller's
+            return fail(AWA_ERR_CUDA, "awa_cache_create: %s", cudaGetErrorString(err));
+        }
+        if (at.type == cudaMemoryTypeUnregistered)
+            return fail(AWA_ERR_INVALID, "awa_cache_create: memory that the GPU cannot reach");
+        if (at.type == cudaMemoryTypeDevice && at.device != device)
+            return fail(AWA_ERR_INVALID, "awa_cache_create: the memory lies on device %d but device %d is current",
+                        at.device, device);
+    }
+    return AWA_OK;
+}
+
 int create(const awa_cache_params* params, awa_cache** out, bool on_device)
 {
     if (!params || !out)
@@ -172,7 +197,15 @@ int create(const awa_cache_params* params, awa_cache** out, bool on_device)
     {
         cudaError_t err = cudaGetDevice(&cache->device);
         if (err == cudaSuccess)
+        {
+            const int memory_rc = check_memory(*params, cache->device);
+            if (memory_rc)
+            {
+                delete cache;
+                return memory_rc;
+            }
             err = static_cast<cudaError_t>(awa::prepare_cache_attention_simt());
+        }
         if (err == cudaSuccess)
             err = static_cast<cudaError_t>(awa::prepare_cache_attention_f32());
         if (err == cudaSuccess)

@@ -30,3 +30,59 @@ def test_strides_of_page_tables_that_are_taken():
     # the stride of a single row is never used
     one = torch.zeros(4, **INTS).expand(1, -1).as_strided((1, 4), (0, 1))
     assert awa_b200.CacheBatch(starts[:2], past[:1], one, 3, 1).c.table_stride == 4
+
+
+def test_pages_in_host_memory_are_refused():
+    k = torch.zeros(6, 2, 16, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        awa_b200.KvCache(k, k.clone())
+
+
+class OnDevice:
+    """A tensor's stand-in that lies on a GPU that need not be there."""
+
+    def __init__(self, index):
+        self.device, self.dtype, self.shape = torch.device("cuda", index), torch.bfloat16, (6, 2, 16, 128)
+
+    def dim(self):
+        return 4
+
+    def stride(self, i=None):
+        strides = (2 * 16 * 128, 16 * 128, 128, 1)
+        return strides if i is None else strides[i]
+
+    def data_ptr(self):
+        return 4096
+
+
+def test_a_handle_is_made_on_the_device_of_its_pages(monkeypatch):
+    """awa_cache_create takes the current device: the pages' one has to be that."""
+    from awa_b200 import cache as binding
+
+    current, made_on = [0], []
+
+    class Device:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    class Library:
+        def awa_cache_create(self, params, handle):
+            made_on.append(current[-1])
+            return 0
+
+        def awa_cache_destroy(self, handle):
+            pass
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(binding, "_lib", Library())
+    cache = awa_b200.KvCache(OnDevice(1), OnDevice(1))
+    assert made_on == [1] and current == [0]
+    assert cache.device.index == 1
+    with pytest.raises(ValueError, match="one device"):
+        awa_b200.KvCache(OnDevice(1), OnDevice(0))
