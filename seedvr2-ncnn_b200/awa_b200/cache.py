@@ -310,6 +310,8 @@ class KvCache:
                 workspace = self._empty(need, _torch().uint8, stream)
             elif workspace.device != self.device:
                 raise ValueError(f"the workspace is on {workspace.device}, the cache on {self.device}")
+            elif not workspace.is_contiguous():
+                raise ValueError("the workspace must be contiguous")
             space, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         rc = self._lib.awa_cache_attention(self._handle, batch.ref, heads, self._type, q.data_ptr(), qs,
                                            self._scale if scale is None else scale, sinks, window, frame_tokens,

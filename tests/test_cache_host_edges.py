@@ -86,3 +86,46 @@ def test_a_handle_is_made_on_the_device_of_its_pages(monkeypatch):
     assert cache.device.index == 1
     with pytest.raises(ValueError, match="one device"):
         awa_b200.KvCache(OnDevice(1), OnDevice(0))
+
+
+def host_cache(storage="bf16", pages=6, heads=2, page=16, dim=128):
+    shape = (pages, heads, page)
+    with torch.device("meta"):  # never read: pages of any number cost nothing
+        if storage == "int4":
+            tensors = [torch.empty(shape + (dim // 2,), dtype=torch.uint8) for _ in range(2)]
+            tensors += [torch.empty(shape + (dim // 64, 2), dtype=torch.bfloat16) for _ in range(2)]
+        else:
+            tensors = [torch.empty(shape + (dim,), dtype=torch.bfloat16) for _ in range(2)]
+    return awa_b200.KvCache(*(Meta(t) for t in tensors), host_only=True)
+
+
+class Meta:
+    """A meta tensor with an address."""
+
+    def __init__(self, t):
+        self._t = t
+        self.device, self.dtype, self.shape, self.stride, self.dim = t.device, t.dtype, t.shape, t.stride, t.dim
+
+    def data_ptr(self):
+        return 4096
+
+
+def host_batch(sequences, width, rows, max_rows, device="meta"):
+    with torch.device(device):
+        return awa_b200.CacheBatch(torch.empty(sequences + 1, **INTS), torch.empty(sequences, **INTS),
+                                   torch.empty(sequences, width, **INTS), rows, max_rows)
+
+
+@pytest.mark.parametrize("make", [
+    lambda n: torch.zeros(1, dtype=torch.uint8).expand(n),
+    lambda n: torch.zeros(4 * n, dtype=torch.uint8)[::4],
+    lambda n: torch.zeros(n // 256, 1, dtype=torch.uint8).expand(-1, 257),
+], ids=["expanded", "strided", "rows"])
+def test_workspaces_with_less_memory_than_elements(make):
+    k = torch.zeros(6, 2, 16, 128, dtype=torch.bfloat16)
+    cache, batch = awa_b200.KvCache(k, k, host_only=True), host_batch(1, 6, 90, 90, "cpu")
+    need = cache.attention_workspace_bytes(batch, 4)
+    assert need > 0
+    q = torch.zeros(90, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="contiguous"):
+        cache.attention(batch, q, workspace=make(need + 256))
