@@ -118,6 +118,8 @@ struct Maps
 };
 
 // ---------------------------------------------------------------- waits and copies
+// Codes of the waits: 70 and 73 to 92. 71 and 72 are AWA_CACHE_BAD_PAGE and AWA_CACHE_BAD_COORD.
+static_assert(AWA_CACHE_BAD_PAGE == 71 && AWA_CACHE_BAD_COORD == 72, "the waits' codes stay clear of these");
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* error_flag,
                                          int code)
 {
@@ -526,7 +528,7 @@ __device__ void clean_role(const CacheAttnArgs& a, Tile<D>& sh)
     int ragged = 0;
     for (int jobs = 0;; jobs++)
     {
-        if (!warp_wait(&sh.job_full[jobs & 1], (jobs >> 1) & 1, abort, a.error_flag, 71))
+        if (!warp_wait(&sh.job_full[jobs & 1], (jobs >> 1) & 1, abort, a.error_flag, 79))
             return;
         const Job& job = sh.job[jobs & 1];
         if (job.t.b < 0)

@@ -3,6 +3,10 @@ kernel sees them, and what a call asks for: no GPU needed."""
 
 from __future__ import annotations
 
+import glob
+import os
+import re
+
 import pytest
 import torch
 
@@ -129,3 +133,14 @@ def test_workspaces_with_less_memory_than_elements(make):
     q = torch.zeros(90, 4, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="contiguous"):
         cache.attention(batch, q, workspace=make(need + 256))
+
+
+def test_no_wait_reports_the_code_of_a_bad_batch():
+    """A wait that ran out must not look like a bad page or coordinate."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    codes = set()
+    for path in glob.glob(os.path.join(root, "seedvr2-ncnn_b200", "csrc", "*.cu")):
+        for line in open(path):
+            codes.update(int(c) for c in re.findall(r"(?:error_flag|wait\(.*),\s*(\d\d)\)", line))
+    assert {73, 79, 80, 92, 31, 61} <= codes  # the sources were understood
+    assert not codes & {awa_b200.AWA_CACHE_BAD_PAGE, awa_b200.AWA_CACHE_BAD_COORD}
