@@ -398,9 +398,10 @@ static int64_t most_pages(const awa::CacheMemory& mem, const awa::CacheBatch& ba
     if (window == 0)
         return all;
     const auto pages = [&](int64_t tokens) { return (tokens + (1 << mem.page_shift) - 1) >> mem.page_shift; };
-    // a row's window and its frame, then rows - 1 more of them, ragged at both ends
-    const int64_t some = batch.sequences * (pages(sinks) + pages((int64_t)window * frame_tokens) + pages(frame_tokens) + 3) +
-                         pages(batch.rows);
+    // a row's window and its frame, ragged at both ends; then rows - 1 more of them
+    int64_t each = pages(sinks) + pages((int64_t)window * frame_tokens) + pages(frame_tokens) + 3;
+    each = each < batch.table_width ? each : batch.table_width;
+    const int64_t some = batch.sequences * each + pages(batch.rows);
     return some < all ? some : all;
 }
 

@@ -114,10 +114,9 @@ class Meta:
         return 4096
 
 
-def host_batch(sequences, width, rows, max_rows, device="meta"):
-    with torch.device(device):
-        return awa_b200.CacheBatch(torch.empty(sequences + 1, **INTS), torch.empty(sequences, **INTS),
-                                   torch.empty(sequences, width, **INTS), rows, max_rows)
+def host_batch(sequences, width, rows, max_rows):
+    return awa_b200.CacheBatch(torch.empty(sequences + 1, **INTS), torch.empty(sequences, **INTS),
+                               torch.empty(sequences, width, **INTS), rows, max_rows)
 
 
 @pytest.mark.parametrize("make", [
@@ -127,7 +126,7 @@ def host_batch(sequences, width, rows, max_rows, device="meta"):
 ], ids=["expanded", "strided", "rows"])
 def test_workspaces_with_less_memory_than_elements(make):
     k = torch.zeros(6, 2, 16, 128, dtype=torch.bfloat16)
-    cache, batch = awa_b200.KvCache(k, k, host_only=True), host_batch(1, 6, 90, 90, "cpu")
+    cache, batch = awa_b200.KvCache(k, k, host_only=True), host_batch(1, 6, 90, 90)
     need = cache.attention_workspace_bytes(batch, 4)
     assert need > 0
     q = torch.zeros(90, 4, 128, dtype=torch.bfloat16)
@@ -144,3 +143,14 @@ def test_no_wait_reports_the_code_of_a_bad_batch():
             codes.update(int(c) for c in re.findall(r"(?:error_flag|wait\(.*),\s*(\d\d)\)", line))
     assert {73, 79, 80, 92, 31, 61} <= codes  # the sources were understood
     assert not codes & {awa_b200.AWA_CACHE_BAD_PAGE, awa_b200.AWA_CACHE_BAD_COORD}
+
+
+@pytest.mark.parametrize("window,frame", [(2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31 - 1, 1), (1, 2 ** 31 - 1), (2 ** 20, 2 ** 30)])
+@pytest.mark.parametrize("sinks", [0, 2 ** 31 - 1])
+@pytest.mark.parametrize("sequences", [1, 33, 64, 5000])
+@pytest.mark.parametrize("storage", ["bf16", "int4"])
+def test_a_window_without_end_needs_no_more_than_none(window, frame, sinks, sequences, storage):
+    """Any product of window and frame is taken: past the table's reach it is all the same."""
+    cache, batch = host_cache(storage), host_batch(sequences, 40, 90 * sequences, 90)
+    most = cache.attention_workspace_bytes(batch, 4)
+    assert 0 < cache.attention_workspace_bytes(batch, 4, sinks, window, frame) <= most
