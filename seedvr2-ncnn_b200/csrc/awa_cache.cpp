@@ -353,13 +353,13 @@ static int check_attention(const char* what, const awa_cache* cache, const awa_c
     return AWA_OK;
 }
 
-// No tile of max_rows rows sees more keys than this: the page table's reach,
-// and the prefix and the window.
+// No max_rows rows of a sequence see more keys than this: the page table's reach,
+// and the prefix, a row's window and what the rows after it add, up to the end of a frame.
 static int64_t most_seen(const awa::CacheMemory& mem, const awa_cache_batch& batch, int sinks, int window,
                          int frame_tokens)
 {
     const int64_t reach = (int64_t)batch.table_width << mem.page_shift;
-    const int64_t seen = sinks + (int64_t)window * frame_tokens + batch.max_rows;
+    const int64_t seen = sinks + (int64_t)window * frame_tokens + batch.max_rows + frame_tokens - 1;
     return window > 0 && seen < reach ? seen : reach;
 }
 

@@ -154,3 +154,11 @@ def test_a_window_without_end_needs_no_more_than_none(window, frame, sinks, sequ
     cache, batch = host_cache(storage), host_batch(sequences, 40, 90 * sequences, 90)
     most = cache.attention_workspace_bytes(batch, 4)
     assert 0 < cache.attention_workspace_bytes(batch, 4, sinks, window, frame) <= most
+
+
+def test_rows_at_a_frame_s_edge_count_both_frames():
+    """A window of one frame of 1200: two rows either side of an edge see 2400 keys, more
+    than a cluster of blocks is for (2048), so the parts of several blocks need a workspace."""
+    cache, batch = host_cache(), host_batch(1, 1000, 2, 2)
+    assert cache.attention_workspace_bytes(batch, 2, 0, 1, 1200) > 0
+    assert cache.attention_workspace_bytes(batch, 2, 0, 1, 900) == 0  # 1800 keys
