@@ -111,6 +111,8 @@ int check_batch(const char* what, const awa_cache* cache, const awa_cache_batch*
     {
         if (!batch->row_starts || !batch->past || !batch->page_table)
             return fail(AWA_ERR_INVALID, "%s: NULL row_starts, past or page_table", what);
+        if (!aligned(batch->row_starts, 0, 4) || !aligned(batch->past, 0, 4) || !aligned(batch->page_table, 0, 4))
+            return fail(AWA_ERR_INVALID, "%s: row_starts, past and page_table must be 4-byte aligned", what);
         if (batch->table_stride < batch->table_width)
             return fail(AWA_ERR_INVALID, "%s: table_stride smaller than table_width", what);
     }
@@ -267,6 +269,8 @@ int awa_cache_append(const awa_cache* cache, const awa_cache_batch* batch, int q
             return fail(AWA_ERR_INVALID,
                         "awa_cache_append: rope needs an 8-byte aligned table, 1 to 4 axes and 2 * axes * pairs <= "
                         "head_dim");
+        if (!aligned(rope->coords, 0, 4))
+            return fail(AWA_ERR_INVALID, "awa_cache_append: rope's coords must be 4-byte aligned");
         a.table = reinterpret_cast<const float2*>(rope->table);
         a.max_coord = rope->max_coord;
         a.axes = rope->axes;

@@ -3,6 +3,7 @@ kernel sees them, and what a call asks for: no GPU needed."""
 
 from __future__ import annotations
 
+import ctypes
 import glob
 import os
 import re
@@ -11,6 +12,7 @@ import pytest
 import torch
 
 import awa_b200
+from awa_b200 import cache as binding
 
 INTS = dict(dtype=torch.int32)
 
@@ -61,8 +63,6 @@ class OnDevice:
 
 def test_a_handle_is_made_on_the_device_of_its_pages(monkeypatch):
     """awa_cache_create takes the current device: the pages' one has to be that."""
-    from awa_b200 import cache as binding
-
     current, made_on = [0], []
 
     class Device:
@@ -162,3 +162,23 @@ def test_rows_at_a_frame_s_edge_count_both_frames():
     cache, batch = host_cache(), host_batch(1, 1000, 2, 2)
     assert cache.attention_workspace_bytes(batch, 2, 0, 1, 1200) > 0
     assert cache.attention_workspace_bytes(batch, 2, 0, 1, 900) == 0  # 1800 keys
+
+
+@pytest.mark.parametrize("field", ["row_starts", "past", "page_table", "coords"])
+@pytest.mark.parametrize("off", [1, 2])
+def test_index_arrays_off_their_alignment(field, off):
+    """A kernel's load from such an address would fault."""
+    lib, P = awa_b200.library(), 4096
+    cache = host_cache()
+    arrays = dict(row_starts=P, past=P, page_table=P, coords=P)
+    arrays[field] += off
+    batch = binding._CacheBatch(2, 5, 3, arrays["row_starts"], arrays["past"], arrays["page_table"], 4, 4)
+    rope = binding._CacheRope(P, 9, 3, 21, arrays["coords"])
+    calls = [lib.awa_cache_append(cache._handle, ctypes.byref(batch), 0, 1, None, 0, P, 256, P, 256,
+                                  ctypes.byref(rope), 1, None, 0, None)]
+    if field != "coords":
+        calls += [lib.awa_cache_read(cache._handle, ctypes.byref(batch), 1, P, 256, P, 256, None),
+                  lib.awa_cache_attention(cache._handle, ctypes.byref(batch), 4, 1, P, 512, 1.0, 0, 0, 1, P, 512, None, 0,
+                                          None)]
+    assert calls == [awa_b200.AWA_ERR_INVALID] * len(calls)
+    assert "aligned" in lib.awa_last_error().decode()
