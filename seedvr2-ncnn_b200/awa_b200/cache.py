@@ -23,6 +23,8 @@ AWA_CACHE_GROUP = 64  # features that share a scale and a minimum in a 4-bit cac
 AWA_CACHE_BAD_PAGE = 71
 AWA_CACHE_BAD_COORD = 72
 
+_INTS = 2 ** 31  # a C int holds -_INTS .. _INTS - 1
+
 # Every symbol declared in include/awa_cache.h.
 CACHE_SYMBOLS = (
     "awa_cache_create", "awa_cache_create_host", "awa_cache_destroy", "awa_cache_append", "awa_cache_read",
@@ -80,6 +82,12 @@ def _current_raw_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
 
 
+def _check_mask(sinks, window, frame_tokens):
+    """ctypes cuts an int to 32 bits; what is left could be a valid mask."""
+    if not (-_INTS <= sinks < _INTS and -_INTS <= window < _INTS and -_INTS <= frame_tokens < _INTS):
+        raise ValueError(f"sinks ({sinks}), window ({window}) and frame_tokens ({frame_tokens}) must fit 32 bits")
+
+
 def rope_table(max_coord: int, pairs: int, base: float = 10000.0, device="cuda"):
     """[max_coord, pairs, 2] fp32 (cos, sin) of coord * base^(-i / pairs), the
     angles in float64 (exact where fp32 angles of far positions are not)."""
@@ -130,6 +138,8 @@ class CacheBatch:
             raise ValueError("row_starts, past and page_table must be on one device")
         self.row_starts, self.past, self.page_table = row_starts, past, page_table
         self.rows, self.device = int(rows), past.device
+        if not (0 <= rows < _INTS and 0 <= max_rows < _INTS):
+            raise ValueError(f"rows ({rows}) and max_rows ({max_rows}) must be 0 or more and fit 32 bits")
         # a single row's stride is never used, but has to hold a row
         width = page_table.shape[1]
         self.c = _CacheBatch(past.shape[0], self.rows, int(max_rows), row_starts.data_ptr(), past.data_ptr(),
@@ -283,6 +293,7 @@ class KvCache:
 
     def attention_workspace_bytes(self, batch: CacheBatch, q_heads: int, sinks: int = 0, window: int = 0,
                                   frame_tokens: int = 1) -> int:
+        _check_mask(sinks, window, frame_tokens)
         return int(self._lib.awa_cache_attention_workspace_bytes(self._handle, batch.ref, q_heads, sinks, window,
                                                                  frame_tokens))
 
@@ -292,6 +303,7 @@ class KvCache:
         1 / sqrt(head_dim) by default): [rows, q_heads, head_dim]. A workspace
         given must not be in use by another call; one made here is not shared."""
         handle = self._stream(batch, stream)
+        _check_mask(sinks, window, frame_tokens)
         if q.dtype != self._rows_dtype:
             raise TypeError(f"this cache takes {self._rows_dtype} rows")
         qs, heads = self._rows(batch, q, "q"), q.shape[1]

@@ -182,3 +182,22 @@ def test_index_arrays_off_their_alignment(field, off):
                                           None)]
     assert calls == [awa_b200.AWA_ERR_INVALID] * len(calls)
     assert "aligned" in lib.awa_last_error().decode()
+
+
+@pytest.mark.parametrize("name", ["sinks", "window", "frame_tokens"])
+@pytest.mark.parametrize("value", [2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63 - 1, -2 ** 32 + 1])
+def test_masks_that_do_not_fit_an_int(name, value):
+    """ctypes would cut them to 32 bits: a prefix of 2^32 + 4 rows to one of 4."""
+    cache, batch = host_cache(), host_batch(1, 6, 2, 2)
+    k = torch.zeros(6, 2, 16, 128, dtype=torch.bfloat16)
+    small = awa_b200.KvCache(k, k, host_only=True)
+    with pytest.raises(ValueError, match=name):
+        small.attention(batch, torch.zeros(2, 4, 128, dtype=torch.bfloat16), **{name: value})
+    with pytest.raises(ValueError, match=name):
+        cache.attention_workspace_bytes(batch, 4, **{name: value})
+
+
+def test_row_counts_that_do_not_fit_an_int():
+    for rows, most in ((2 ** 32 + 2, 2), (2, 2 ** 32 + 2), (2, 2 ** 31)):
+        with pytest.raises(ValueError, match="rows"):
+            host_batch(1, 6, rows, most)
