@@ -409,12 +409,18 @@ static int64_t most_pages(const awa::CacheMemory& mem, const awa::CacheBatch& ba
     return some < all ? some : all;
 }
 
-// The workspace of kUnpackTile ahead of the tile kernel's: keys, values, page table, queries, each on 256 bytes.
+// The workspace of kUnpackTile ahead of the tile kernel's: keys, values, page table,
+// queries, ranges and the scores' scales, each on 256 bytes.
 struct Unpacked
 {
     int64_t pages;
-    size_t page_bytes, pool_bytes, table_bytes, q_bytes;
+    size_t page_bytes, pool_bytes, table_bytes, q_bytes, range_bytes, scale_bytes;
 };
+
+static size_t on256(size_t bytes)
+{
+    return (bytes + 255) / 256 * 256;
+}
 
 static Unpacked unpacked_of(const awa::CacheMemory& mem, const awa::CacheBatch& batch, int q_heads, int sinks,
                             int window, int frame_tokens)
@@ -423,8 +429,10 @@ static Unpacked unpacked_of(const awa::CacheMemory& mem, const awa::CacheBatch& 
     u.pages = most_pages(mem, batch, sinks, window, frame_tokens);
     u.page_bytes = ((size_t)mem.heads * mem.head_dim * 2) << mem.page_shift;
     u.pool_bytes = u.pages * u.page_bytes;
-    u.table_bytes = ((size_t)batch.sequences * batch.table_width * 4 + 255) / 256 * 256;
-    u.q_bytes = ((size_t)batch.rows * q_heads * mem.head_dim * 2 + 255) / 256 * 256;
+    u.table_bytes = on256((size_t)batch.sequences * batch.table_width * 4);
+    u.q_bytes = on256((size_t)batch.rows * q_heads * mem.head_dim * 2);
+    u.range_bytes = on256((size_t)mem.heads * (mem.head_dim / AWA_CACHE_GROUP) * 2 * sizeof(unsigned));
+    u.scale_bytes = on256((size_t)batch.rows * q_heads * sizeof(float));
     return u;
 }
 
@@ -448,7 +456,7 @@ size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cac
     if (kernel == kTile)
         return parts;
     const Unpacked u = unpacked_of(cache->mem, b, q_heads, sinks, window, frame_tokens);
-    return 2 * u.pool_bytes + u.table_bytes + u.q_bytes + parts;
+    return 2 * u.pool_bytes + u.table_bytes + u.q_bytes + u.range_bytes + u.scale_bytes + parts;
 }
 
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,
@@ -526,6 +534,9 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
         unpack.q_stride = q_token_stride;
         unpack.q_row = (int)row;
         unpack.pages = (int)u.pages;
+        unpack.ranges = reinterpret_cast<unsigned*>(unpack.q_out + u.q_bytes);
+        unpack.score_scale = reinterpret_cast<float*>(reinterpret_cast<char*>(unpack.ranges) + u.range_bytes);
+        unpack.scale = scale;
         unpack.error_flag = a.error_flag;
         err = awa::launch_cache_unpack(unpack, s);
         if (err)
@@ -540,7 +551,9 @@ int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, in
         a.batch.table_stride = a.batch.table_width;
         a.q = unpack.q_out;
         a.q_stride = row;
-        err = awa::launch_cache_attention_tile(a, true, unpack.q_out + u.q_bytes, s);
+        a.ranges = unpack.ranges;
+        a.score_scale = unpack.score_scale;
+        err = awa::launch_cache_attention_tile(a, true, reinterpret_cast<char*>(unpack.score_scale) + u.scale_bytes, s);
         break;
     }
     }

@@ -9,6 +9,7 @@
 // measured copy rate); 8 rows 3.9 us.
 #include "awa_cache_device.cuh"
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,6 +30,7 @@ struct PageSlot
 {
     int b;  // -1: none
     int entry;
+    int lo, hi;  // the rows of the sequence see its positions [0, sinks) and [lo, hi)
 };
 
 __device__ __forceinline__ PageSlot find_page(const CacheUnpackArgs& a, int index)
@@ -41,15 +43,18 @@ __device__ __forceinline__ PageSlot find_page(const CacheUnpackArgs& a, int inde
         const int b = base + lane;
         KeyBlocks pages;
         pages.prefix = pages.shift = pages.count = 0;
+        RowSpan first = {0, 0}, last = {0, 0};
         if (b < a.batch.sequences)
         {
             const int rows = batch_rows(a.batch, b);
             const int past = max(0, __ldg(a.batch.past + b));
             const int length = sequence_length(a.mem, a.batch, past, rows, nullptr);
             if (rows > 0)
-                pages = key_blocks(row_span(min(past, length), length, a.sinks, a.window, a.frame_tokens),
-                                   row_span(min(past, length) + rows - 1, length, a.sinks, a.window, a.frame_tokens),
-                                   a.sinks, page);
+            {
+                first = row_span(min(past, length), length, a.sinks, a.window, a.frame_tokens);
+                last = row_span(min(past, length) + rows - 1, length, a.sinks, a.window, a.frame_tokens);
+                pages = key_blocks(first, last, a.sinks, page);
+            }
         }
         int sum = pages.count;
 #pragma unroll
@@ -66,11 +71,12 @@ __device__ __forceinline__ PageSlot find_page(const CacheUnpackArgs& a, int inde
             const int i = index - before - __shfl_sync(0xffffffffu, sum - pages.count, src);
             const int prefix = __shfl_sync(0xffffffffu, pages.prefix, src);
             const int shift = __shfl_sync(0xffffffffu, pages.shift, src);
-            return {base + src, i < prefix ? i : i + shift};
+            return {base + src, i < prefix ? i : i + shift, __shfl_sync(0xffffffffu, first.lo, src),
+                    __shfl_sync(0xffffffffu, last.hi, src)};
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    return {-1, 0};
+    return {-1, 0, 0, 0};
 }
 
 // 8 consecutive elements, in 16-byte pieces where the rows allow it.
@@ -137,12 +143,16 @@ __device__ __forceinline__ void quantize8(const float (&v)[8], uint32_t& codes, 
     params = (__float_as_uint(scale) >> 16) | (__float_as_uint(minimum) & 0xffff0000u);
 }
 
-__device__ __forceinline__ void dequantize8(uint32_t codes, uint32_t params, float (&v)[8])
+__device__ __forceinline__ void dequantize8(uint32_t codes, float scale, float minimum, float (&v)[8])
 {
-    const float scale = __uint_as_float(params << 16), minimum = __uint_as_float(params & 0xffff0000u);
 #pragma unroll
     for (int i = 0; i < 8; i++)
         v[i] = __fadd_rn(__fmul_rn((float)((codes >> (4 * i)) & 15u), scale), minimum);
+}
+
+__device__ __forceinline__ void dequantize8(uint32_t codes, uint32_t params, float (&v)[8])
+{
+    dequantize8(codes, __uint_as_float(params << 16), __uint_as_float(params & 0xffff0000u), v);
 }
 
 // 8 consecutive elements as they are loaded: raw 16-byte pieces where the rows
@@ -427,6 +437,130 @@ __device__ __forceinline__ uint4 half8(const float (&v)[8])
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The largest magnitudes that the minimum and scale of a group allow, of what
+// some row sees, per head and 64 features. A cluster per head: its warps take the
+// pages in turn, lanes the slots of a page. Its blocks join in shared memory: no
+// zeros to begin with, no atomics.
+constexpr int kRangeBlocks = 8, kRangeThreads = 512, kRangeWarps = kRangeThreads / 32;
+
+template <int GROUPS>
+__global__ void __cluster_dims__(kRangeBlocks) __launch_bounds__(kRangeThreads) cache_range_kernel(CacheUnpackArgs a)
+{
+    __shared__ unsigned most_s[kRangeWarps][2 * GROUPS];
+    __shared__ unsigned block_s[2 * GROUPS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const CacheMemory& mem = a.mem;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, page_tokens = 1 << mem.page_shift;
+    const int64_t head = blockIdx.y * mem.params_head_stride;
+    float most[2 * GROUPS] = {};  // k, v of each group
+    for (int i = blockIdx.x * kRangeWarps + warp; i < a.pages; i += kRangeBlocks * kRangeWarps)
+    {
+        const PageSlot at = find_page(a, i);
+        if (at.b < 0)
+            break;
+        const int page = __ldg(a.batch.page_table + at.b * a.batch.table_stride + at.entry);
+        if ((unsigned)page >= (unsigned)mem.pages)
+            continue;  // reported where it is unpacked
+        for (int slot = lane; slot < page_tokens; slot += 32)
+        {
+            const int key = (at.entry << mem.page_shift) + slot;
+            if (!(key < at.hi && (key >= at.lo || key < a.sinks)))
+                continue;
+            const int64_t from = page * mem.params_page_stride + head + (int64_t)slot * GROUPS * 4;
+#pragma unroll
+            for (int g = 0; g < 2 * GROUPS; g++)
+            {
+                const uint32_t params =
+                    __ldg(reinterpret_cast<const uint32_t*>((g & 1 ? mem.v_params : mem.k_params) + from) + (g >> 1));
+                const float scale = __uint_as_float(params << 16), low = __uint_as_float(params & 0xffff0000u);
+                most[g] = fmaxf(most[g], fmaxf(fabsf(low), fabsf(fmaf(15.f, scale, low))));
+            }
+        }
+    }
+    // floats that are not negative are ordered as their bits are
+#pragma unroll
+    for (int g = 0; g < 2 * GROUPS; g++)
+    {
+        const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most[g]));
+        if (lane == 0)
+            most_s[warp][g] = bits;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2 * GROUPS)
+    {
+        unsigned bits = 0;
+        for (int w = 0; w < kRangeWarps; w++)
+            bits = max(bits, most_s[w][threadIdx.x]);
+        block_s[threadIdx.x] = bits;
+    }
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    if (blockIdx.x == 0 && threadIdx.x < 2 * GROUPS)
+    {
+        unsigned bits = 0;
+        for (int r = 0; r < kRangeBlocks; r++)
+            bits = max(bits, *cluster.map_shared_rank(&block_s[threadIdx.x], r));
+        a.ranges[(int64_t)blockIdx.y * 2 * GROUPS + threadIdx.x] = bits;
+    }
+    cluster.sync();  // a block's shared memory stays until it has been read
+}
+
+// Ends when cache_range_kernel, beside which the unpacking starts, has ended.
+__device__ __forceinline__ void wait_for_ranges()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+__device__ __forceinline__ int shift_of(const CacheUnpackArgs& a, int kv, int group, bool is_k)
+{
+    // not __ldg: written while this kernel may have been there already
+    return half_shift(
+        __ldcg(a.ranges + ((int64_t)kv * (a.mem.head_dim / AWA_CACHE_GROUP) + group) * 2 + (is_k ? 0 : 1)));
+}
+
+// 8 features of q a thread; the head_dim / 8 lanes of one head and row, which
+// stand side by side, share its power of two.
+__device__ __forceinline__ void unpack_queries(const CacheUnpackArgs& a, int64_t first, int64_t step)
+{
+    const int d = a.mem.head_dim, shift = d == 64 ? 6 : 7, heads = a.q_row >> shift, lanes = d / 8;
+    const int per_kv = heads / a.mem.heads;
+    const int64_t chunks = a.q_row / 8, all = chunks * a.batch.rows;
+    const int lane = threadIdx.x & 31;
+    for (int64_t i = first; i - lane < all; i += step)
+    {
+        const bool mine = i < all;
+        const int64_t row = mine ? i / chunks : 0;
+        const int f = mine ? (int)(i - row * chunks) * 8 : 0;  // of the row
+        float v[8] = {};
+        if (mine)
+            load8(static_cast<const bf16*>(a.q) + row * a.q_stride + f, v);
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            most = fmaxf(most, fabsf(v[j]));
+        const int head = f >> shift;
+        const int down = shift_of(a, head / per_kv, (f & (d - 1)) / AWA_CACHE_GROUP, true);
+        int top = most > 0.f ? (int)(__float_as_uint(most) >> 23) - 127 - down : -1024;
+        for (int o = 1; o < lanes; o <<= 1)
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int up = top == -1024 ? 0 : 14 - top;
+        // in two factors: one may be outside the floats' range
+        const int n0 = max(-126, min(127, up - down)), n1 = max(-126, min(127, up - down - n0));
+        const float by0 = power_of_two(n0), by1 = power_of_two(n1);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            v[j] = v[j] * by0 * by1;
+        if (!mine)
+            continue;
+        reinterpret_cast<uint4*>(a.q_out)[i] = half8(v);
+        // never 0 or infinite, which would make NaN of a masked or an empty score; so
+        // far out, scores are next to 0 or beyond the floats
+        if ((f & (d - 1)) == 0)
+            a.score_scale[row * heads + head] =
+                fminf(fmaxf(ldexpf(a.scale * 1.4426950408889634f, -up), 0x1p-126f), 0x1p127f);
+    }
+}
+
 // One 4-bit page that some row of the batch sees -> its keys and values as fp16
 // (rounded by 2^-12, where bf16's 2^-9 of every key would show in the scores),
 // and its number in the workspace's page table. Blocks: x = the pages of all
@@ -434,19 +568,13 @@ __device__ __forceinline__ uint4 half8(const float (&v)[8])
 __global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs a)
 {
     __shared__ int which_s[2];
+    __shared__ float up_s[4];  // powers of two: keys and values of each group
     const CacheMemory& mem = a.mem;
     if ((int)blockIdx.x >= a.pages)
     {
-        const int64_t chunks = a.q_row / 8, all = chunks * a.batch.rows;
-        const int64_t step = (int64_t)(gridDim.x - a.pages) * gridDim.y * kThreads;
-        int64_t i = ((int64_t)(blockIdx.x - a.pages) * gridDim.y + blockIdx.y) * kThreads + threadIdx.x;
-        for (; i < all; i += step)
-        {
-            const int64_t row = i / chunks;
-            float v[8];
-            load8(static_cast<const bf16*>(a.q) + row * a.q_stride + (i - row * chunks) * 8, v);
-            reinterpret_cast<uint4*>(a.q_out)[i] = half8(v);
-        }
+        wait_for_ranges();
+        unpack_queries(a, ((int64_t)(blockIdx.x - a.pages) * gridDim.y + blockIdx.y) * kThreads + threadIdx.x,
+                       (int64_t)(gridDim.x - a.pages) * gridDim.y * kThreads);
         return;
     }
     if (threadIdx.x < 32)
@@ -457,6 +585,13 @@ __global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs 
             which_s[0] = at.b;
             which_s[1] = at.entry;
         }
+    }
+    else if (threadIdx.x < 64)  // beside it
+    {
+        wait_for_ranges();  // every block: the grid must not end ahead of that kernel
+        const int i = threadIdx.x - 32;
+        if (i < 2 * (mem.head_dim / AWA_CACHE_GROUP))
+            up_s[i] = power_of_two(shift_of(a, blockIdx.y, i >> 1, (i & 1) == 0));
     }
     __syncthreads();
     const int b = which_s[0], entry = which_s[1];
@@ -475,11 +610,12 @@ __global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs 
     const int64_t src = page * mem.page_stride + kv * mem.head_stride;
     const int64_t par = page * mem.params_page_stride + kv * mem.params_head_stride;
     const int64_t dst = ((int64_t)blockIdx.x * mem.heads + kv) * page_bytes * 4;
+    const int pieces = (int)(page_bytes / 8);  // of the keys, then as many of the values
     // 16 codes, of one group, a thread and turn
-    for (int i = threadIdx.x; i < 2 * (int)(page_bytes / 8); i += kThreads)
+    for (int i = threadIdx.x; i < 2 * pieces; i += kThreads)
     {
-        const bool is_k = i < (int)(page_bytes / 8);
-        const int at = (is_k ? i : i - (int)(page_bytes / 8)) * 8;
+        const bool is_k = i < pieces;
+        const int at = (is_k ? i : i - pieces) * 8;
         uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (real)
         {
@@ -487,10 +623,14 @@ __global__ void __launch_bounds__(kThreads) cache_unpack_kernel(CacheUnpackArgs 
             const int row = at / row_bytes, group = (at - row * row_bytes) / (AWA_CACHE_GROUP / 2);
             const uint32_t params = __ldg(
                 reinterpret_cast<const uint32_t*>((is_k ? mem.k_params : mem.v_params) + par) + row * groups + group);
+            // scaled ahead of the products: the same roundings
+            const float by = up_s[2 * group + (is_k ? 0 : 1)];
+            const float scale = __uint_as_float(params << 16) * by;
+            const float minimum = __uint_as_float(params & 0xffff0000u) * by;
             float v[8];
-            dequantize8(codes.x, params, v);
+            dequantize8(codes.x, scale, minimum, v);
             out[0] = half8(v);
-            dequantize8(codes.y, params, v);
+            dequantize8(codes.y, scale, minimum, v);
             out[1] = half8(v);
         }
         uint4* to = reinterpret_cast<uint4*>((is_k ? a.k_out : a.v_out) + dst + (int64_t)at * 4);
@@ -596,11 +736,27 @@ int launch_cache_read(const CacheReadArgs& a, int out_dtype, cudaStream_t stream
 int launch_cache_unpack(const CacheUnpackArgs& a, cudaStream_t stream)
 {
     ProfileScope scope("awa_cache_unpack", stream);
+    const dim3 clusters(kRangeBlocks, (unsigned)a.mem.heads);
+    if (a.mem.head_dim == AWA_CACHE_GROUP)
+        cache_range_kernel<1><<<clusters, kRangeThreads, 0, stream>>>(a);
+    else
+        cache_range_kernel<2><<<clusters, kRangeThreads, 0, stream>>>(a);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess)
+        return (int)err;
     // 4 pieces of q a thread
-    const int64_t pieces = (int64_t)a.batch.rows * (a.q_row / 8);
-    const int64_t q_blocks = (pieces + 4 * kThreads * a.mem.heads - 1) / (4 * kThreads * a.mem.heads);
-    cache_unpack_kernel<<<dim3((unsigned)(a.pages + q_blocks), (unsigned)a.mem.heads), kThreads, 0, stream>>>(a);
-    return (int)cudaGetLastError();
+    const int64_t pieces = (int64_t)a.batch.rows * (a.q_row / 8), at_once = (int64_t)4 * kThreads * a.mem.heads;
+    const int64_t q_blocks = (pieces + at_once - 1) / at_once;
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    config.stream = stream;
+    config.gridDim = dim3((unsigned)(a.pages + q_blocks), (unsigned)a.mem.heads);
+    config.blockDim = dim3(kThreads);
+    return (int)cudaLaunchKernelEx(&config, cache_unpack_kernel, a);
 }
 
 }  // namespace awa

@@ -919,10 +919,13 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem,
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + kColS + 128 * x + lane_base;
     const uint32_t t_o = tmem + kColO + 128 * x + lane_base;
-    const float scale_log2 = a.scale * 1.4426950408889634f;
+    float scale_log2 = a.scale * 1.4426950408889634f;
     volatile int* abort = &sh.abort;
     // whole sectors at a time, where the rows are aligned to them
     const bool v8 = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_stride * sizeof(bf16))) & 31) == 0;
+    // fp16 ends at 2^-24: with the largest p at 2^7 to 2^15, what is below 2^-32 of
+    // it is dropped instead of 2^-25 (bf16 has fp32's exponents)
+    constexpr float kHeadroom = HALF ? 7.f : 0.f;
     uint32_t phase = 0;
     for (int jobs = 0;; jobs++)
     {
@@ -934,9 +937,13 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem,
         const int m_tile = job.rows_per_tile * a.group;
         const int m = job.t.m0 + x * m_tile + min(r, m_tile - 1);
         const bool mine = r < m_tile && x * m_tile + r < job.t.count;
+        if (HALF)
+            scale_log2 = mine ? __ldg(a.score_scale + (int64_t)(job.t.row0 + m / a.group) * (a.group * a.mem.heads) +
+                                      job.kv * a.group + m % a.group)
+                              : 1.f;
         const RowSpan span =
             row_span(job.t.past + m / a.group, job.t.length, a.sinks, a.window, a.frame_tokens);
-        float m_run = -INFINITY;  // running maximum, in log2 units of the scaled scores
+        float m_run = -INFINITY;  // running maximum, in log2 units of the scaled scores, less kHeadroom
         float l_run = 0.f;
         bool any = false;
         const KeyBlocks blocks = job.blocks;
@@ -978,7 +985,7 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem,
 #pragma unroll
             for (int j = 0; j < kKeys / 2; j++)
                 top[j & 3] = max3(top[j & 3], __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-            const float m_blk = max3(max3(top[0], top[1], top[2]), top[3], -INFINITY) * scale_log2;
+            const float m_blk = max3(max3(top[0], top[1], top[2]), top[3], -INFINITY) * scale_log2 - kHeadroom;
             // O is scaled only when the maximum has grown by more than 2^8: until
             // then the larger exponentials stay well inside fp32 and bf16
             float alpha = 1.f;
@@ -1039,14 +1046,14 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem,
         }
         // Epilogue: O divided by the sums as bf16 or, of a job that other thread
         // blocks share, as it is.
-        const int slot = job.slot;
+        const int slot = job.slot, kv = job.kv;
         if (slot >= 0 && mine)
             part_ml[((int64_t)slot * 2 + x) * kRows + r] = make_float2(m_run, l_run);
         // a row that sees nothing (l = 0) gets zeros
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         char* const row =
             reinterpret_cast<char*>(static_cast<bf16*>(a.out) + (int64_t)(job.t.row0 + m / a.group) * a.out_stride +
-                                    (int64_t)(job.kv * a.group + m % a.group) * D);
+                                    (int64_t)(kv * a.group + m % a.group) * D);
         float* const sum = part_o + (((int64_t)slot * 2 + x) * kRows + r) * D;
         __syncwarp();
         if ((threadIdx.x & 31) == 0)
@@ -1072,6 +1079,15 @@ __device__ void softmax_role(const CacheAttnArgs& a, Tile<D>& sh, uint32_t tmem,
         mbar_arrive(&sh.o_empty[x]);
         if (!mine)
             continue;
+        if (HALF)  // the power of two of the unpacked values
+#pragma unroll
+            for (int c = 0; c < D / 64; c++)
+            {
+                const float down = power_of_two(-half_shift(__ldg(a.ranges + (kv * (D / 64) + c) * 2 + 1)));
+#pragma unroll
+                for (int j = 64 * c; j < 64 * c + 64; j++)
+                    o[j] = __float_as_uint(__uint_as_float(o[j]) * down);
+            }
         if (slot >= 0)
         {
 #pragma unroll

@@ -14,6 +14,18 @@ __device__ __forceinline__ void cache_error(int* flag, int code)
         atomicCAS(flag, 0, code);
 }
 
+// n for the 2^n that brings numbers up to the one with these bits below 2^15,
+// for use as fp16 operands: -114 to 126, so that 2^n and 2^-n are normal floats.
+__device__ __forceinline__ int half_shift(unsigned bits)
+{
+    return 14 - max((int)(bits >> 23) - 127, -112);
+}
+
+__device__ __forceinline__ float power_of_two(int n)  // -126 to 127
+{
+    return __int_as_float((n + 127) << 23);
+}
+
 // Sequence whose rows contain `row` (largest b with row_starts[b] <= row), or
 // -1 if it belongs to nobody. Empty sequences share their start with the next.
 __device__ __forceinline__ int sequence_of_row(const CacheBatch& batch, int row)

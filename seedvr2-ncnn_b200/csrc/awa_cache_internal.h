@@ -68,7 +68,11 @@ struct CacheReadArgs
 
 // 4-bit pages that a batch sees -> dense fp16 pages [page][head][slot][head_dim]
 // and a page table [sequences][table_width] of theirs; the batch's q rows, bf16
-// -> dense fp16.
+// -> dense fp16. fp16 keeps 11 bits of numbers from 2^-14 to 2^16 only, so all of
+// it is scaled by powers of two: the keys and the values of a head's 64 features
+// to below 2^15 (half_shift() of their largest, in `ranges`), a row of q to below
+// 2^15 after it has taken the keys' powers back. score_scale: what the products
+// of a row's scores are multiplied by, `scale` log2(e) and those powers.
 struct CacheUnpackArgs
 {
     CacheMemory mem;
@@ -80,6 +84,9 @@ struct CacheUnpackArgs
     int64_t q_stride;
     int q_row;  // elements of a row
     int pages;  // as many as the batch can see, at most
+    unsigned* ranges;    // [heads][head_dim / 64][k, v]: bits of the largest magnitude that some row sees
+    float* score_scale;  // [rows][q heads]
+    float scale;
     int* error_flag;
 };
 
@@ -94,6 +101,8 @@ struct CacheAttnArgs
     int64_t out_stride;
     float scale;
     int sinks, window, frame_tokens;
+    const unsigned* ranges;    // of what launch_cache_unpack wrote
+    const float* score_scale;
     int* error_flag;
 };
 

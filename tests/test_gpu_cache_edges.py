@@ -10,6 +10,7 @@ import torch
 
 import awa_b200
 from awa_b200 import cache as binding
+from cache_testlib import Batch, quantize, seen_keys, unpack
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +35,156 @@ def test_memory_that_the_gpu_cannot_reach_is_refused():
     for k, v in ((pointer, on_gpu.data_ptr()), (on_gpu.data_ptr(), pointer)):
         rc, error = create(k, v)
         assert rc == awa_b200.AWA_ERR_INVALID and "GPU" in error
+
+
+# ---------------------------------------------------------------- 4 bits, as close as the kernels are
+def four_bit_attention(c, q, sinks, window, frame, scale, many):
+    """(out, tolerance) of a 4-bit cache in float64, row by row.
+
+    A row of values is minimum + scale * code; with K^ = |minimum| + scale * code
+    for keys, V^ for values, p the probabilities, d features, n keys:
+      few rows: codes are exact operands, so scores carry fp32 sums of d products
+        of both parts: (d + 4) 2^-24 sum |q| K^. p times the scale is rounded to
+        bf16 once: 2^-8 p |v|. The sums over n keys: n 2^-24 p V^. A scale
+        below 2^-80 max(1, |minimum|) is raised to that, which moves a value by up
+        to 15 2^-80 max(1, |minimum|), and products whose share of the result is
+        below 2^-126 / (2^-133 2^90) = 2^-83 may be cut: together 2^-75
+        max(1, |minimum|) a key, weighed by p (at most 1) and by 1 for n < 2^8 keys.
+      many rows: keys, values and p in fp16: 2^-11 sum |q k| on the scores, 2^-11
+        twice on p |v| (q, 8 bits, is exact); p below 2^-32 of the row's largest
+        is dropped: 2^-31 V^ a key. The sums as above.
+    exp2: 2^-22, the division 2^-23; out: half a step of bf16."""
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    group = q.shape[1] // c.kv_heads
+    for b, (n, p) in enumerate(zip(c.rows, c.past)):
+        if not n:
+            continue
+        k, v, k_up, v_up = (x.repeat_interleave(group, 1) for x in
+                            (c.cached(b, "k"), c.cached(b, "v"), magnitude(c, b, "k"), magnitude(c, b, "v")))
+        r = slice(c.first[b], c.first[b] + n)
+        x = q[r].double()
+        seen = torch.stack([seen_keys(p + i, n + p, sinks, window, frame) for i in range(n)]).to(q.device)
+        s = torch.einsum("ihd,jhd->hij", x, k) * scale
+        prob = torch.softmax(s.masked_fill(~seen, float("-inf")), -1).nan_to_num(0.0)
+        top = lambda y: (torch.einsum("ihd,jhd->hij", x.abs(), y) * scale).masked_fill(~seen, 0).amax(-1)
+        out[r] = torch.einsum("hij,jhd->ihd", prob, v)
+        a, a_up = (torch.einsum("hij,jhd->ihd", prob, y) for y in (v.abs(), v_up))
+        score = (c.d + 4) * 2.0 ** -24 * top(k_up) + (2.0 ** -11 * top(k.abs()) if many else 0)
+        tol[r] = a * (2 * 2.0 ** -11 if many else 2.0 ** -8) + a_up * (2.0 ** -22 + (n + p + 8) * 2.0 ** -24)
+        tol[r] += a_up * 2 * torch.expm1(score).T[..., None] + 2.0 ** -8 * out[r].abs() + 1e-37
+        if not many:
+            tol[r] += 2.0 ** -75 * max(1.0, v_up.max().item()) * (1 + (n + p) / 256)
+        if many:
+            most = prob.amax(-1).T[..., None]
+            tol[r] += 2.0 ** -31 * most * torch.einsum("hij,jhd->ihd", seen[None].expand_as(prob).double(), v_up)
+    return out, tol
+
+
+def magnitude(c, b, name):
+    page, slot = c.slots(b, torch.arange(c.rows[b] + c.past[b]))
+    params = c.params[0 if name == "k" else 1][page, :, slot].abs()
+    return unpack(getattr(c, name)[page, :, slot], params).double()
+
+
+def fill_four_bit(c, k, v):
+    """The rows [past + rows, heads, d] of c's only sequence, packed."""
+    page, slot = c.slots(0, torch.arange(k.shape[0]))
+    for t, p, x in ((c.k, c.params[0], k), (c.v, c.params[1], v)):
+        t[page, :, slot], p[page, :, slot] = quantize(x)
+
+
+def check_four_bit(c, q, sinks=0, window=0, frame=1, scale=None, most=0.003):
+    """most: of the error's norm, relative to the result's. bf16's rounding of
+    the output is up to 2^-8 / sqrt(3) = 0.0023 of it; keys and values rounded to
+    bf16 would come to 0.0048."""
+    cache, batch = c.handles(awa_b200)
+    scale = c.d ** -0.5 if scale is None else scale
+    out = cache.attention(batch, q, sinks=sinks, window=window, frame_tokens=frame, scale=scale)
+    torch.cuda.synchronize()
+    awa_b200.device_status()
+    many = max(c.rows) * (q.shape[1] // c.kv_heads) > 32
+    want, tol = four_bit_attention(c, q[:c.total], sinks, window, frame, scale, many)
+    out = out[:c.total].double()
+    assert not out.isnan().any()
+    off = (out - want).abs()
+    assert (off <= tol).all(), f"{(off / tol).max().item():.3g} of the tolerance"
+    if most and (many or want.abs().max() > 2.0 ** -60):
+        assert (off.norm() <= most * want.norm()), f"{(off.norm() / want.norm()).item():.3g} of the norm"
+        # the bound tells these from the result
+        assert (want.abs() > tol).any() and (2 * want.abs() > tol).float().mean() > 0.5
+
+
+ROWS = [1, 8, 9, 150]  # 8 rows of a group of 4: the last that the kernel for few rows takes
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("size_k,size_v,size_q", [
+    (1, 1, 1), (1e-4, 1, 1e4), (1, 1e-4, 1), (1e-6, 1e-6, 1e6), (1e-8, 1e-8, 1e6), (1, 1e-12, 1), (1, 1e-30, 1),
+    (3e4, 3e4, 1e-4), (1e4, 1, 1e-4), (1, 1, 1e-3)])
+def test_four_bit_values_of_any_size(size_k, size_v, size_q, rows, d):
+    """What a row gets does not depend on how many rows come with it, for tiny values as well."""
+    c = Batch([rows], [200], 16, 2, d, "int4", seed=21)
+    x = torch.randn(2, 200 + rows, 2, d, generator=c.generator).cuda()
+    fill_four_bit(c, size_k * x[0], size_v * x[1])
+    q = (size_q * c.new_rows(8, torch.float32)).bfloat16()
+    check_four_bit(c, q, window=150, sinks=3, scale=min(1.0, 1 / (size_k * size_q)) * d ** -0.5)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_four_bit_groups_of_different_sizes(rows):
+    """Heads, groups of 64 features and rows of q far apart in size."""
+    c = Batch([rows], [120], 32, 2, 128, "int4", seed=22)
+    x = torch.randn(2, 120 + rows, 2, 128, generator=c.generator).cuda()
+    x[0, :, 0, :64] *= 1e-7
+    x[0, :, 1, 64:] *= 1e3
+    x[1, :, 0, 64:] *= 1e-9
+    x[1, :, 1, :64] *= 1e4
+    fill_four_bit(c, x[0], x[1])
+    q = c.new_rows(8, torch.float32)
+    q[..., :64] *= torch.tensor([1e7, 1.0]).repeat_interleave(4)[:, None].cuda()
+    q[..., 64:] *= torch.tensor([1.0, 1e-3]).repeat_interleave(4)[:, None].cuda()
+    q[::3] *= 1e-5
+    check_four_bit(c, q.bfloat16())
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("below", [20, 24, 27, 30])
+def test_four_bit_keys_far_below_the_largest(below, rows):
+    """One key holds all but 2^-below of a row, and 0 as its value: the others make the result."""
+    c = Batch([rows], [300], 16, 1, 64, "int4", seed=23)
+    k = torch.zeros(300 + rows, 1, 64, device="cuda")
+    v = 1 + torch.rand(300 + rows, 1, 64, generator=c.generator).cuda()
+    k[5], v[5] = 1.0, 0.0
+    fill_four_bit(c, k, v)
+    q = torch.full((rows, 4, 64), below / 64, device="cuda").bfloat16()  # exact: a multiple of 2^-6 below 2^8
+    check_four_bit(c, q, scale=0.6931471805599453, most=0.005)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("sinks,window,frame", [(0, 0, 1), (20, 90, 1), (20, 2, 33)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_four_bit_attention_as_close_as_it_is(d, sinks, window, frame, rows):
+    c = Batch([rows, 0, max(1, rows // 2)], [400, 7, 33], 16, 2, d, "int4", seed=24, extra_rows=2)
+    check_four_bit(c, 1.5 * c.new_rows(8, torch.bfloat16), sinks, window, frame)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_four_bit_peaked_softmax(rows):
+    c = Batch([rows], [500], 32, 2, 128, "int4", seed=25)
+    check_four_bit(c, 1.5 * c.new_rows(2 if rows == 1 else 8, torch.bfloat16), scale=0.5, most=0)
+
+
+def test_four_bit_sequences_of_different_sizes():
+    """The largest values of one sequence take nothing from another's."""
+    c = Batch([60, 50, 40], [100, 30, 77], 16, 2, 128, "int4", seed=26)
+    for b, (k_size, v_size) in enumerate(((1.0, 1.0), (1e-3, 1e-6), (30.0, 1e4))):
+        page, slot = c.slots(b, torch.arange(c.rows[b] + c.past[b]))
+        for t, p, size in ((c.k, c.params[0], k_size), (c.v, c.params[1], v_size)):
+            x = size * torch.randn(page.shape[0], 2, 128, generator=c.generator).cuda()
+            t[page, :, slot], p[page, :, slot] = quantize(x)
+    q = c.new_rows(8, torch.float32)
+    q[60:110] *= 1e3
+    q[110:] *= 0.03
+    check_four_bit(c, q.bfloat16(), most=0)
