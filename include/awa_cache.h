@@ -153,10 +153,14 @@ int awa_cache_read(const awa_cache* cache, const awa_cache_batch* batch, int out
  * have to be finite; with an AWA_INT4 cache they and q are of fp16's range,
  * below 65504 (its products run on fp16 operands where there are many rows).
  * workspace: awa_cache_attention_workspace_bytes() bytes, 256-byte aligned
- * (NULL if that is 0), used by this call until its work is done: calls that may overlap, two captured graphs among them, need one each.
- * It holds the parts of rows that several blocks work on (few rows, long
- * caches) and, for many rows over an AWA_INT4 cache, q and the visible pages
- * as fp16 (rounded once); other calls need none. */
+ * (NULL if that is 0), used by this call until its work is done: calls that may
+ * overlap, two captured graphs among them, need one each. It holds the parts of
+ * rows that several blocks work on (few rows of long caches, many rows: tens of
+ * MB) and, for many rows over an AWA_INT4 cache, q and the visible pages as fp16
+ * (rounded once): as many pages as the table reaches within window and prefix,
+ * but no more than the cache has, of as many heads at a time as 2 GiB hold (of
+ * one, if one head's are more). AWA_F32 caches and head sizes other than 64 and
+ * 128 need none. */
 size_t awa_cache_attention_workspace_bytes(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int sinks,
                                            int window, int frame_tokens);
 int awa_cache_attention(const awa_cache* cache, const awa_cache_batch* batch, int q_heads, int dtype, const void* q,

@@ -66,9 +66,10 @@ struct CacheReadArgs
     int* error_flag;
 };
 
-// 4-bit pages that a batch sees -> dense fp16 pages [page][head][slot][head_dim]
-// and a page table [sequences][table_width] of theirs; the batch's q rows, bf16
-// -> dense fp16. fp16 keeps 11 bits of numbers from 2^-14 to 2^16 only, so all of
+// 4-bit pages that a batch sees -> dense fp16 pages [page][head][slot][head_dim];
+// the batch's q rows, bf16 -> dense fp16. The pages take the numbers that they
+// have in the cache, or those in which the sequences see them, with a page table
+// [sequences][table_width]: whichever needs room for fewer. fp16 keeps 11 bits of numbers from 2^-14 to 2^16 only, so all of
 // it is scaled by powers of two: the keys and the values of a head's 64 features
 // to below 2^15 (half_shift() of their largest, in `ranges`), a row of q to below
 // 2^15 after it has taken the keys' powers back. score_scale: what the products
@@ -79,12 +80,13 @@ struct CacheUnpackArgs
     CacheBatch batch;
     int sinks, window, frame_tokens;
     char *k_out, *v_out, *q_out;
-    int* table;
+    int* table;  // NULL: the pages keep their numbers
     const void* q;
     int64_t q_stride;
     int q_row;  // elements of a row
-    int pages;  // as many as the batch can see, at most
+    int most_seen;  // pages of all sequences together, at most
     unsigned* ranges;    // [heads][head_dim / 64][k, v]: bits of the largest magnitude that some row sees
+    unsigned* range_parts;  // cache_unpack_range_bytes()
     float* score_scale;  // [rows][q heads]
     float scale;
     int* error_flag;
@@ -108,6 +110,7 @@ struct CacheAttnArgs
 
 int launch_cache_append(const CacheAppendArgs& args, int in_dtype, int q_out_dtype, cudaStream_t stream);
 int launch_cache_read(const CacheReadArgs& args, int out_dtype, cudaStream_t stream);
+size_t cache_unpack_range_bytes(const CacheMemory& mem, int heads);
 int launch_cache_unpack(const CacheUnpackArgs& args, cudaStream_t stream);
 // fp32 and bf16 caches of any head_dim, fp32 arithmetic.
 int launch_cache_attention_simt(const CacheAttnArgs& args, int max_rows, cudaStream_t stream);

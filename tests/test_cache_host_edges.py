@@ -201,3 +201,23 @@ def test_row_counts_that_do_not_fit_an_int():
     for rows, most in ((2 ** 32 + 2, 2), (2, 2 ** 32 + 2), (2, 2 ** 31)):
         with pytest.raises(ValueError, match="rows"):
             host_batch(1, 6, rows, most)
+
+
+GIB = 2 ** 30
+
+
+@pytest.mark.parametrize("pages,heads,page,sequences,width", [
+    (2000, 8, 64, 64, 512),      # streams of a few hundred tokens with room for 32768 in the table
+    (100, 2, 16, 1000, 4000),
+    (40000, 8, 64, 64, 512),     # a cache that could be full of what they see
+    (1000000, 20, 64, 3, 300000),
+    (5000, 1, 256, 200, 4096),
+])
+def test_workspace_of_many_rows_over_4_bits(pages, heads, page, sequences, width):
+    """Pools of fp16 pages: never more of them than the cache has, and those of as
+    many heads at a time as 1 GiB holds (one, if one head's are more)."""
+    cache = host_cache("int4", pages, heads, page)
+    batch = host_batch(sequences, width, 9 * sequences, 9)
+    one_head = min(pages, sequences * width) * page * 128 * 2 * 2
+    beside = sequences * width * 4 + 9 * sequences * 4 * heads * (128 * 2 + 4) + (80 << 20)  # table, q, parts of rows
+    assert cache.attention_workspace_bytes(batch, 4 * heads) <= max(min(2 * GIB, heads * one_head), one_head) + beside

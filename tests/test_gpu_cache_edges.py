@@ -188,3 +188,47 @@ def test_four_bit_sequences_of_different_sizes():
     q[60:110] *= 1e3
     q[110:] *= 0.03
     check_four_bit(c, q.bfloat16(), most=0)
+
+
+@pytest.mark.parametrize("width", [700, 840])  # x 3 sequences: fewer pages than the cache has, and more
+def test_four_bit_heads_in_several_passes(width):
+    """Unpacked pages of more than 2 GiB: some heads at a time. The table has room
+    for far more rows than there are."""
+    pages, heads = 2500, 10
+    c = Batch([40, 3, 30], [600, 300, 0], 256, heads, 128, "int4", seed=27, extra_rows=1)
+    for name in ("k", "v"):
+        x = torch.zeros((pages,) + getattr(c, name).shape[1:], dtype=torch.uint8, device="cuda")
+        x[:getattr(c, name).shape[0]] = getattr(c, name)
+        setattr(c, name, x)
+    params = []
+    for p in c.params:
+        x = torch.full((pages,) + p.shape[1:], float("nan"), dtype=p.dtype, device="cuda")
+        x[:p.shape[0]] = p
+        params.append(x)
+    c.params = tuple(params)
+    c.table = torch.nn.functional.pad(c.table, (0, width - c.table.shape[1]), value=2 ** 31 - 1)
+    cache, batch = c.handles(awa_b200)
+    need = cache.attention_workspace_bytes(batch, 4 * heads)
+    assert need < 2 ** 31 < heads * min(pages, 3 * width) * 256 * 128 * 4
+    check_four_bit(c, 1.5 * c.new_rows(4 * heads, torch.bfloat16), sinks=5, most=0.003)
+
+
+def test_four_bit_pages_shared_by_sequences():
+    """More table entries than pages: the unpacked ones are the cache's, whoever sees them."""
+    c = Batch([40, 40, 40], [96, 96, 96], 16, 2, 64, "int4", seed=28)
+    c.table[1:, :6] = c.table[0, :6]  # a common prefix
+    c.table = torch.nn.functional.pad(c.table, (0, 100), value=-1)
+    check_four_bit(c, 1.5 * c.new_rows(8, torch.bfloat16))
+    # a page that the cache does not have counts as zero keys and values, and is reported
+    page = c.table[2, 7].item()
+    c.table[2, 7] = c.k.shape[0]
+    cache, batch = c.handles(awa_b200)
+    q = c.new_rows(8, torch.bfloat16)
+    got = cache.attention(batch, q)
+    with pytest.raises(awa_b200.AwaError, match="71"):
+        awa_b200.device_status()
+    c.table[2, 7] = page
+    for p in c.params:
+        p[page] = 0
+    want, tol = four_bit_attention(c, q, 0, 0, 1, 64 ** -0.5, True)
+    assert ((got.double() - want).abs() <= tol).all()
