@@ -10,7 +10,8 @@ import torch
 
 import awa_b200
 from awa_b200 import cache as binding
-from cache_testlib import Batch, quantize, seen_keys, unpack
+import test_gpu_cache as others
+from cache_testlib import Batch, attention, quantize, rotate, seen_keys, unpack
 
 pytestmark = pytest.mark.gpu
 
@@ -232,3 +233,130 @@ def test_four_bit_pages_shared_by_sequences():
         p[page] = 0
     want, tol = four_bit_attention(c, q, 0, 0, 1, 64 ** -0.5, True)
     assert ((got.double() - want).abs() <= tol).all()
+
+
+# ---------------------------------------------------------------- sizes
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+def test_append_of_many_rows(storage):
+    """9472 rows and more go 16 to a block; the last tile is short."""
+    others.test_append_bit_exact(([9500, 3], [37, 0], 64, 2, 3, 128, 3, 21), torch.bfloat16, storage)
+
+
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+@pytest.mark.parametrize("rows", [1, 2, 40])
+def test_groups_of_more_than_128_heads(rows, storage):
+    c = Batch([rows, 1], [70, 200], 16, 1, 64, storage, seed=31, extra_rows=1)
+    others.attend(c, 130, 4, 100, 1, torch.float32 if storage == "f32" else torch.bfloat16)
+
+
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_more_than_16384_sequences(rows, storage):
+    """Most of them without rows; those that have some are spread."""
+    sequences = 16500
+    has = [rows if b % 700 == 5 else 0 for b in range(sequences)]
+    past = [37 * (b % 5) if n else 0 for b, n in enumerate(has)]
+    c = Batch(has, past, 16, 1, 64, storage, seed=32)
+    others.attend(c, 2, 0, 60, 1, torch.float32 if storage == "f32" else torch.bfloat16)
+
+
+def side_by_side(c):
+    """Keys and values, and their params, of a page next to one another."""
+    both, params = torch.stack([c.k, c.v], 1), torch.stack(c.params, 1)
+    c.k, c.v, c.params = both[:, 0], both[:, 1], (params[:, 0], params[:, 1])
+
+
+def heads_outside(c):
+    """The pages of a head next to one another."""
+    turn = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    c.k, c.v, c.params = turn(c.k), turn(c.v), tuple(turn(p) for p in c.params)
+
+
+@pytest.mark.parametrize("layout", [side_by_side, heads_outside])
+@pytest.mark.parametrize("rows", [[1, 2], [60, 3]])
+@pytest.mark.parametrize("d", [64, 128])
+def test_four_bit_layouts(d, rows, layout):
+    c = Batch(rows, [130, 77], 16, 3, d, "int4", seed=33)
+    layout(c)
+    check_four_bit(c, 1.5 * c.new_rows(6, torch.bfloat16), sinks=3, window=90)
+    cache, batch = c.handles(awa_b200)
+    k, v = (c.new_rows(3, torch.bfloat16) for _ in range(2))
+    cache.append(batch, k, v)
+    back = cache.read(batch, torch.float32)
+    for x, got in ((k, back[0]), (v, back[1])):
+        assert torch.equal(got, unpack(*quantize(x.float())))
+
+
+# ---------------------------------------------------------------- beside the framework's other operators
+def test_append_turns_rows_as_mmrope_does():
+    """With the layer's own angles, row by row the same bits."""
+    plan = awa_b200.AwaPlan(2, 4, 6, 1, 1, 1)
+    info = plan.info
+    text, n, heads = info.text_tokens, info.source_tokens, 2
+    x = torch.randn(n, 3, heads, 128, device="cuda")
+    t = torch.randn(text, 3, heads, 128, device="cuda")
+    packed, starts = plan.pack(x, t)
+    starts = starts.int().tolist()
+    turned = plan.mmrope(packed)
+    unit = torch.zeros_like(packed)
+    unit[..., 0::2] = 1.0  # comes back as (cos, sin)
+    angles = plan.mmrope(unit)[:, 0, 0, :126].view(-1, 3, 21, 2)
+    for window in range(info.window_count):
+        rows = slice(starts[window], starts[window + 1])
+        count = rows.stop - rows.start
+        # a table with one entry for each row and axis
+        table = angles[rows].reshape(count * 3, 21, 2).contiguous()
+        coords = torch.arange(3 * count, dtype=torch.int32, device="cuda").view(count, 3).contiguous()
+        c = Batch([count], [0], 64, heads, 128, "f32", seed=34)
+        cache, batch = c.handles(awa_b200)
+        q, k, v = packed[rows].unbind(1)
+        got = cache.append(batch, k, v, q=q, rope=awa_b200.CacheRope(table, coords))
+        back = cache.read(batch)
+        want = turned[rows]
+        assert torch.equal(got, want[:, 0]) and torch.equal(back[0], want[:, 1]) and torch.equal(back[1], want[:, 2])
+    awa_b200.device_status()
+
+
+@pytest.mark.parametrize("storage", ["bf16", "int4"])
+def test_frames_from_projection_to_projection(storage):
+    """A block's step over a stream: QKV projection, append, attention, output projection; text, then frames."""
+    heads, d, model, text, frame, page = 3, 128, 192, 10, 40, 16
+    g = torch.Generator().manual_seed(35)
+    normal = lambda *shape: torch.randn(*shape, generator=g).cuda()
+    w_in, w_out = (normal(3 * heads * d, model) / model ** 0.5).bfloat16(), (normal(256, heads * d) / 20).bfloat16()
+    gamma_q, gamma_k, bias, gate = 1 + 0.2 * normal(d), 1 + 0.2 * normal(d), 0.1 * normal(256), 0.2 * normal(256)
+    cache = awa_b200.KvCache.empty(30, page, heads, d, storage)
+    table = torch.randperm(30, generator=g).int().cuda()[None]
+    angles = awa_b200.rope_table(64, 21)
+    c = Batch([0], [0], page, heads, d, storage)
+    c.k, c.v, c.params, c.table = cache.k, cache.v, (cache.k_params, cache.v_params), table
+    past = 0
+    for step in range(4):
+        n = text if step == 0 else frame
+        x, residual = normal(n, model).bfloat16(), normal(n, 256).bfloat16()
+        qkv = awa_b200.qkv_project(x, w_in, gamma_q, gamma_k, 1e-5, heads)
+        q, k, v = qkv.unbind(1)  # views: rows 3 * heads * d apart
+        i = torch.arange(n, device="cuda", dtype=torch.int32)
+        coords = torch.stack([i, i, i] if step == 0 else [0 * i + text + step, i // 8, i % 8], 1).contiguous()
+        batch = awa_b200.CacheBatch(torch.tensor([0, n], dtype=torch.int32, device="cuda"),
+                                    torch.tensor([past], dtype=torch.int32, device="cuda"), table, n, n)
+        turned = cache.append(batch, k, v, q=q, rope=awa_b200.CacheRope(angles, coords))
+        assert torch.equal(turned, rotate(q, angles, coords).bfloat16())
+        out = cache.attention(batch, turned, sinks=text, window=2, frame_tokens=frame)
+        got = awa_b200.out_project(out.flatten(1), w_out, bias, gate, residual)
+        awa_b200.device_status()
+        c.rows, c.past, c.first, c.total = [n], [past], [0, n], n
+        if storage == "int4":
+            want, tol = four_bit_attention(c, turned, text, 2, frame, d ** -0.5, n * 1 > 32)
+        else:
+            want, tol = attention(c, turned, text, 2, frame, d ** -0.5)
+        assert ((out.double() - want).abs() <= tol).all(), step
+        # the projection of these rows: products exact in fp32, sums of heads * d of them, two
+        # roundings to bf16 (product, output) of up to 2^-8 each
+        y = out.flatten(1).double() @ w_out.double().T + bias
+        size = out.flatten(1).double().abs() @ w_out.double().abs().T + bias.abs()
+        final = residual.double() + y * gate
+        bound = gate.abs() * (2.0 ** -8 * y.abs() + heads * d * 2.0 ** -23 * size) + 2.0 ** -8 * final.abs()
+        bound += 2.0 ** -22 * (residual.double().abs() + (y * gate).abs()) + 2.0 ** -8 * bound
+        assert ((got.double() - final).abs() <= bound).all(), step
+        past += n
