@@ -51,8 +51,8 @@ typedef struct awa_cache awa_cache;
  * byte i holding feature 2i in its low and 2i + 1 in its high four bits, with
  *   k_params + p * params_page_stride + h * params_head_stride + s * 2 * (head_dim / 64)
  * (bf16 elements): (scale, minimum) of each 64 features. A code c stands for
- * scale * c + minimum in fp32. Bases and strides are multiples of 16 bytes
- * (of 4 bytes for the params). */
+ * scale * c + minimum in fp32. Bases and strides are multiples of 16 bytes,
+ * the strides below 2^40 bytes. */
 typedef struct
 {
     int storage;     /* AWA_F32, AWA_BF16 or AWA_INT4 */

@@ -71,6 +71,11 @@ int check_params(const awa_cache_params& p)
         return fail(AWA_ERR_INVALID, "awa_cache_create: NULL memory");
     const int64_t row = p.storage == AWA_INT4 ? p.head_dim / 2 : p.head_dim;
     const int64_t element = p.storage == AWA_INT4 ? 1 : type_bytes(p.storage);
+    // what tensor maps take, and far from where products of them pass 64 bits
+    const int64_t most = (int64_t)1 << 40;  // bytes
+    if (p.head_stride >= most / element || p.page_stride >= most / element ||
+        (p.storage == AWA_INT4 && (p.params_head_stride >= most / 2 || p.params_page_stride >= most / 2)))
+        return fail(AWA_ERR_INVALID, "awa_cache_create: strides must stay below 2^40 bytes");
     // either order of pages and heads, but no two rows in one place
     const bool fits = p.head_stride >= p.page_tokens * row && p.page_stride >= p.page_tokens * row &&
                       (p.page_stride >= p.heads * p.head_stride || p.head_stride >= p.pages * p.page_stride);

@@ -221,3 +221,23 @@ def test_workspace_of_many_rows_over_4_bits(pages, heads, page, sequences, width
     one_head = min(pages, sequences * width) * page * 128 * 2 * 2
     beside = sequences * width * 4 + 9 * sequences * 4 * heads * (128 * 2 + 4) + (80 << 20)  # table, q, parts of rows
     assert cache.attention_workspace_bytes(batch, 4 * heads) <= max(min(2 * GIB, heads * one_head), one_head) + beside
+
+
+@pytest.mark.parametrize("storage,field", [
+    (s, f + "_stride") for s in ("bf16", "f32", "int4")
+    for f in ("page", "head", *(("params_page", "params_head") if s == "int4" else ()))])
+@pytest.mark.parametrize("value", [2 ** 40, 2 ** 60, 2 ** 62, 2 ** 63 - 2 ** 10])
+def test_strides_that_no_memory_has(storage, field, value):
+    """Their products would pass 64 bits, and tensor maps end at 2^40 bytes."""
+    four = storage == "int4"
+    row = 64 if four else 128
+    p = dict(page_stride=4 * 16 * row, head_stride=16 * row, params_page_stride=4 * 16 * 4, params_head_stride=16 * 4)
+    p[field] = value
+    code = {"bf16": awa_b200.AWA_BF16, "f32": awa_b200.AWA_F32, "int4": awa_b200.AWA_INT4}[storage]
+    params = binding._CacheParams(code, 4, 128, 16, 10, 4096, 4096, p["page_stride"], p["head_stride"],
+                                  4096 if four else None, 4096 if four else None, p["params_page_stride"],
+                                  p["params_head_stride"])
+    handle = ctypes.c_void_p()
+    rc = awa_b200.library().awa_cache_create_host(ctypes.byref(params), ctypes.byref(handle))
+    awa_b200.library().awa_cache_destroy(handle)
+    assert rc == awa_b200.AWA_ERR_INVALID
