@@ -360,3 +360,85 @@ def test_frames_from_projection_to_projection(storage):
         bound += 2.0 ** -22 * (residual.double().abs() + (y * gate).abs()) + 2.0 ** -8 * bound
         assert ((got.double() - final).abs() <= bound).all(), step
         past += n
+
+
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+@pytest.mark.parametrize("rows", [[1, 2], [70, 0, 45]])
+def test_rows_ahead_of_the_first_sequence(rows, storage):
+    """row_starts that begin behind 0: the rows before belong to nobody, as those behind the last."""
+    dtype = torch.float32 if storage == "f32" else torch.bfloat16
+    c = Batch(rows, [60] * len(rows), 16, 2, 128, storage, seed=36)
+    ahead, behind, n = 5, 4, sum(rows)
+    c.starts += ahead
+    q, k, v = (torch.full((ahead + n + behind, h, 128), float("nan"), device="cuda").to(dtype) for h in (4, 2, 2))
+    for t in (q, k, v):
+        t[ahead:ahead + n] = torch.randn(n, t.shape[1], 128, generator=c.generator).to(dtype)
+    cache = awa_b200.KvCache(c.k, c.v, *c.params)
+    batch = awa_b200.CacheBatch(c.starts, c.past_t, c.table, ahead + n + behind, max(rows))
+    table = awa_b200.rope_table(200, 64)
+    turned = torch.full_like(q, 7.0)
+    cache.append(batch, k, v, q=q, rope=awa_b200.CacheRope(table), q_out=turned)
+    out = torch.full_like(q, 5.0)
+    cache.attention(batch, turned, sinks=3, window=50, out=out)
+    awa_b200.device_status()
+    pos = torch.cat([60 + torch.arange(m) for m in rows]).cuda()[:, None]
+    mine = slice(ahead, ahead + n)
+    assert torch.equal(turned[mine], rotate(q[mine], table, pos).to(dtype))
+    for t, kept in ((turned, 7.0), (out, 5.0)):
+        assert (t[:ahead] == kept).all() and (t[ahead + n:] == kept).all()
+    if storage == "int4":
+        want, tol = four_bit_attention(c, turned[mine], 3, 50, 1, 128 ** -0.5, max(rows) * 2 > 32)
+    else:
+        want, tol = attention(c, turned[mine], 3, 50, 1, 128 ** -0.5)
+    assert ((out[mine].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+@pytest.mark.parametrize("most", [1, 100])
+@pytest.mark.parametrize("rows,sequences", [(0, 0), (0, 2), (4, 0), (4, 2)])
+def test_batches_without_work(rows, sequences, most, storage):
+    dtype = torch.float32 if storage == "f32" else torch.bfloat16
+    cache = awa_b200.KvCache.empty(4, 16, 2, 64, storage)
+    for t in (cache.k, cache.v):
+        t.zero_()
+    ints = dict(dtype=torch.int32, device="cuda")
+    batch = awa_b200.CacheBatch(torch.zeros(sequences + 1, **ints), torch.zeros(sequences, **ints),
+                                torch.full((sequences, 3), -1, **ints), rows, most)
+    q, k, v = (torch.ones(rows, h, 64, device="cuda").to(dtype) for h in (4, 2, 2))
+    out = torch.full_like(q, 3.0)
+    turned = cache.append(batch, k, v, q=q, q_out=out.clone())
+    assert cache.attention(batch, q, out=out) is out
+    cache.read(batch)
+    awa_b200.device_status()
+    assert (out == 3.0).all() and (turned == 3.0).all() and not cache.k.any() and not cache.v.any()
+
+
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+@pytest.mark.parametrize("rows", [1, 9, 150])
+def test_lengths_that_change_behind_a_call(rows, storage):
+    """The next step's lengths and rows are written right behind the call, on its stream:
+    kernels that start early must not take them, nor later ones miss them."""
+    dtype = torch.float32 if storage == "f32" else torch.bfloat16
+    c = Batch([rows] * 3, [9000, 4000, 6000], 64, 2, 128, storage, seed=37)
+    for t in ((c.k, c.v) if storage != "int4" else c.params):
+        t.nan_to_num_(0.25)
+    cache, batch = c.handles(awa_b200)
+    q = c.new_rows(8, dtype)
+    pasts = [torch.tensor(p, dtype=torch.int32, device="cuda") for p in
+             ([9000, 4000, 6000], [10, 500, 5900], [8000, 0, 77])]  # within the pages that each has
+    rowss = [q.clone(), q.flip(0).contiguous(), (0.5 * q)]
+    want = []
+    for p, x in zip(pasts, rowss):
+        c.past_t.copy_(p)
+        q.copy_(x)
+        want.append(cache.attention(batch, q, sinks=4))
+        torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for p, x in zip(pasts, rowss):
+            c.past_t.copy_(p)
+            q.copy_(x)
+            got.append(cache.attention(batch, q, sinks=4))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    awa_b200.device_status()
