@@ -18,7 +18,10 @@
  * contents change. What the device finds wrong in them (a page number or a
  * coordinate out of range, a sequence longer than its page table) it reports
  * through awa_device_status(): AWA_CACHE_BAD_PAGE or AWA_CACHE_BAD_COORD; it
- * never reads or writes outside the buffers for it.
+ * never reads or writes outside the buffers for it. Rows without a place are not
+ * appended or read back; to awa_cache_attention the rows of a page that is not
+ * there are keys and values of zeros, which count in the softmax, and a sequence
+ * ends where its page table does.
  */
 #ifndef AWA_CACHE_H
 #define AWA_CACHE_H
@@ -146,12 +149,18 @@ int awa_cache_read(const awa_cache* cache, const awa_cache_batch* batch, int out
  *   A row that sees nothing gets zeros. Pages that no row of the batch sees
  *   need not be there: their page_table entries are not read.
  * q and out: rows x q_heads x head_dim (dense within a row) of AWA_F32 for an
- * AWA_F32 cache (to fp32 accuracy: FFMA or six bf16 products, fp32 sums), else of AWA_BF16
- * (16-bit operands on the tensor cores, fp32 accumulation and softmax
- * statistics). 16-byte aligned rows. scale: > 0. sinks and window: 0 or more,
+ * AWA_F32 cache (to fp32 accuracy: FFMA or six bf16 products, fp32 sums), else of
+ * AWA_BF16 (16-bit operands on the tensor cores: the cache's values and the
+ * probabilities, rounded once to bf16 or, many rows of 4 bits, fp16; fp32
+ * accumulation and softmax statistics, the probabilities' sum taken before that
+ * rounding). 16-byte aligned rows. scale: > 0. sinks and window: 0 or more,
  * frame_tokens: 1 or more. Values in the cache that some row of the batch sees
- * have to be finite; with an AWA_INT4 cache they and q are of fp16's range,
- * below 65504 (its products run on fp16 operands where there are many rows).
+ * have to be finite; with an AWA_INT4 cache they and q are below 65504 in
+ * magnitude. Of those, few rows tell values apart down to 2^-70. Many rows take
+ * them as fp16 (11 bits) scaled by powers of two, one for the keys and one for
+ * the values of each 64 features of a head: 2^-38 of the largest that some row
+ * of the batch sees there is the least they tell apart; probabilities below
+ * 2^-32 of a row's largest are dropped.
  * workspace: awa_cache_attention_workspace_bytes() bytes, 256-byte aligned
  * (NULL if that is 0), used by this call until its work is done: calls that may
  * overlap, two captured graphs among them, need one each. It holds the parts of

@@ -5,8 +5,11 @@
 // pairs of q and k, one rounding to the storage type (or to 4-bit codes with a
 // scale and a minimum per 64 features). Nothing is read or written twice, so
 // memory bounds it: bytes = rows * (q + k + v in, q + k + v out). Measured (B200):
-// 86074 rows of 20 heads of 128 in bf16, 2.64 GB, 466 us (5.7 TB/s, 0.87 of the
-// measured copy rate); 8 rows 3.9 us.
+// 86074 rows of 20 heads of 128 in bf16, 2.64 GB, 480 us (5.5 TB/s, 0.84 of the
+// measured copy rate); 8 rows 3.9 us. Read back, the rows' k and v take 326 us
+// (5.4 TB/s), of an fp32 cache 570 us (6.2 TB/s), of a 4-bit one, to fp32, 406 us
+// (5.0 TB/s); to append them to it takes 448 us (2.5 TB/s): the minimum, maximum
+// and rounding of 64 values a group keep the SMs' issue 0.6 busy.
 #include "awa_cache_device.cuh"
 
 #include <cuda_bf16.h>
@@ -714,7 +717,8 @@ struct Shape
 };
 
 // Heads side by side: the multiple of the cache's heads that leaves the fewest
-// threads idle over q, k and v, at 128 to 512 threads. Few rows: a block each.
+// threads idle over q, k and v, at more than 128 threads, if the heads allow it, and
+// at most 512. Few rows: a block each.
 // More: a block takes several, so that the lookup of sequence, page and
 // coordinates, which its threads wait for, is paid once a tile: 4, and 16 where
 // that still leaves every SM some blocks (86074 rows: 478 us with 4, 455 with

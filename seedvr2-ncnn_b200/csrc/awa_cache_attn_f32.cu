@@ -17,7 +17,7 @@
 // 128 FMAs a clock that the FMA units do, with far fewer loads from shared
 // memory per FMA. Measured (B200): 512 rows of 20 heads over 1594 keys 141 us, 31
 // TFLOP/s of fp32 (236 us with FMAs). The products' own time is 45 us: they keep
-// the tensor pipe 0.46 of the time busy; two warps a scheduler do not cover the
+// the tensor pipe 0.48 of the time busy; two warps a scheduler do not cover the
 // latency of their MMAs, softmax and splitting, and the registers (255) allow no
 // more.
 #include "awa_cache_join.cuh"

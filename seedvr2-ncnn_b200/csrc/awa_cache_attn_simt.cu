@@ -10,11 +10,11 @@
 // The FMA units bound it: 4 d flops per visible pair at 128 FMAs a clock and SM.
 // Both products go through fma.f32x2, two of them per instruction, so that their
 // issue leaves room for the loads from shared memory; two blocks on an SM work
-// under each other's waits. Measured (B200), with 128 features known when
-// compiling: 512 rows of 20 heads over 1594 keys 236 us, 18 TFLOP/s, a quarter of
-// the FMA rate: a tile's 14 blocks of keys are few beside its start, its loads and
-// the uneven last round of blocks. With 64 and 128 features such calls go to the
-// tensor cores (141 us).
+// under each other's waits. Measured (B200): 1024 rows of 32 / 8 heads of 96 over
+// 4096 keys 1.58 ms, 28.5 TFLOP/s, 0.38 of the FMA rate (bf16 1.53 ms). For single
+// rows the loads count, and a block has none in flight while it computes: 64
+// streams of 8192 fp32 keys, 32 / 8 heads of 128, 2.98 ms, 1.4 TB/s; one of 32768
+// keys 555 us (8 blocks a tile, 64 SMs); one of 701 keys, 20 heads, 66 us.
 #include "awa_cache_join.cuh"
 
 #include <cuda_bf16.h>
@@ -61,9 +61,10 @@ __device__ __forceinline__ void mul2(Pair& acc, Pair a)
     asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(a));
 }
 
-// T: type of the cache, q and out. D: head_dim, 0 if only the cache knows it. A block (of a cluster of gridDim.x / tiles that share the keys) takes one
-// tile of R * 16 query rows of one key/value head. Thread (ty, tx) of 16 x 16:
-// rows ty * R + i, keys tx + 16 j, output features 4 (tx + 16 j).
+// T: type of the cache, q and out. D: head_dim, 0 if only the cache knows it. A
+// block (of a cluster of gridDim.x / tiles that share the keys) takes one tile of
+// R * 16 query rows of one key/value head. Thread (ty, tx) of 16 x 16: rows
+// ty * R + i, keys tx + 16 j, output features 4 (tx + 16 j).
 template <typename T, int R, int D>
 __global__ void __launch_bounds__(kThreads, 2) cache_attention_simt_kernel(CacheAttnArgs a, int cluster_size)
 {
@@ -307,8 +308,9 @@ int run(const CacheAttnArgs& a, cudaStream_t stream)
 {
     const int64_t rows = (int64_t)a.batch.rows * a.group;
     const int64_t tiles = rows / (16 * R) + a.batch.sequences;
-    // a start and a join cost about 4 blocks of keys (160 tiles of 14: 291, 236, 244
-    // and 313 us with 1, 2, 4 and 8 blocks a tile)
+    // a start and a join cost about 4 blocks of keys (64 rows of 128 features, before
+    // they went to the tensor cores, 160 tiles of 14: 291, 236, 244 and 313 us with 1,
+    // 2, 4 and 8 blocks a tile)
     const int cluster = cluster_of(a, rows, 16 * R, kKeys, 4.0);
     if (tiles * cluster > 0x7fffffff)
         return (int)cudaErrorInvalidConfiguration;

@@ -26,9 +26,9 @@
 // rounding acts on p as it does for a bf16 cache.
 //
 // Measured (B200): 64 streams of 500 to 32000 rows, window 8192, 32 / 8 heads:
-// 194 us, 6.0 TB/s, 0.92 of the measured copy rate. The same in 4 bits, 32
-// streams up to 32700 rows: 138 us, 4.1 TB/s, 0.63: there the instructions that
-// turn codes into operands (350 a 16 keys and warp) bound it, not memory. One
+// 195 us, 6.0 TB/s, 0.91 of the measured copy rate. The same in 4 bits, 32
+// streams up to 32700 rows: 143 us, 4.0 TB/s, 0.60: there the instructions that
+// turn codes into operands (320 a 16 keys and warp) bound it, not memory. One
 // stream of 700 rows: 8.4 us.
 #include "awa_cache_device.cuh"
 #include "awa_mma.cuh"
@@ -881,7 +881,8 @@ __device__ __forceinline__ QueryTile tile_of(const CacheAttnArgs& a, int b, int 
 // earlier block began) or 2c + 1 (one that a later block ends) of block c, and
 // cache_attention_join_kernel joins them.
 template <int ST, int D, int NQ>
-__global__ void __launch_bounds__(kThreads, ST == AWA_INT4 && NQ == 1 ? 3 : 2) cache_attention_split_kernel(CacheAttnArgs a, float* part_o, float2* part_ml)
+__global__ void __launch_bounds__(kThreads, ST == AWA_INT4 && NQ == 1 ? 3 : 2)
+    cache_attention_split_kernel(CacheAttnArgs a, float* part_o, float2* part_ml)
 {
     using S = Step<ST, D>;
     constexpr int kRows = 8 * NQ;
@@ -1014,7 +1015,9 @@ __global__ void __launch_bounds__(D / 2) cache_attention_join_kernel(CacheAttnAr
     store_out<D>(a, t, kv, r, f, j);
 }
 
-// Blocks of the split kernel: as many as run at once on 148 SMs.
+// Blocks of the split kernel: as many as shared memory lets run at once on 148
+// SMs. Of the 4-bit instances, those with 64 features, or with two tiles, hold
+// fewer for their registers, so that some of their blocks run behind the others.
 template <int ST, int D, int NQ>
 constexpr int split_blocks()
 {

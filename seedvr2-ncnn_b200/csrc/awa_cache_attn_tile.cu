@@ -5,7 +5,8 @@
 //
 // out = softmax(scale q K^T) V in one pass: per block of 128 keys, S = Q K^T
 // into TMEM, the running maximum and sum of each row (base 2, fp32), P =
-// 2^(S - max) in 16 bits over S in TMEM, O += P V into TMEM. 4 d flops per visible
+// 2^(S - max) in 16 bits over S in TMEM, O += P V into TMEM. fp16 operands come
+// scaled by powers of two, which the scores and O take back. 4 d flops per visible
 // pair of query row and key against 4 d bytes per key and 256 rows: the tensor
 // cores and the exponentials bound it, not memory.
 //
@@ -36,10 +37,10 @@
 // 128 keys a block: S_A, S_B, O_A, O_B fill the 512 TMEM columns at head_dim
 // 128, P takes the place of S. Every wait is bounded, as in the window kernel.
 //
-// Measured (B200): 8192 rows of 20 heads over 20538 keys 1.78 ms, 970 TFLOP/s,
-// under the power limit (1.54 ms, 1118 TFLOP/s, with pauses between the calls);
-// 1024 rows over 9274 keys 0.147 ms, 660 TFLOP/s with the unpacking. A key block
-// of both tiles takes about 3500 clocks where the MMAs alone need 2048 and the
+// Measured (B200): 8192 rows of 20 heads over 20538 keys 1.89 ms, 911 TFLOP/s,
+// under the power limit (1.61 ms, 1070 TFLOP/s, with pauses between the calls);
+// 1024 rows over 9274 keys of 4 bits 0.163 ms, 597 TFLOP/s with the unpacking. A key block
+// of both tiles takes about 3300 clocks where the MMAs alone need 2048 and the
 // exponentials 2048: the softmax of a tile (2100-2300 clocks, half of it
 // exponentials) and the MMAs behind it (1050) follow one another, and only two
 // tiles fit TMEM to overlap them. Tried and slower: a quarter of the exponentials

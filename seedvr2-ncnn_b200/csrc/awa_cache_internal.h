@@ -69,11 +69,12 @@ struct CacheReadArgs
 // 4-bit pages that a batch sees -> dense fp16 pages [page][head][slot][head_dim];
 // the batch's q rows, bf16 -> dense fp16. The pages take the numbers that they
 // have in the cache, or those in which the sequences see them, with a page table
-// [sequences][table_width]: whichever needs room for fewer. fp16 keeps 11 bits of numbers from 2^-14 to 2^16 only, so all of
-// it is scaled by powers of two: the keys and the values of a head's 64 features
-// to below 2^15 (half_shift() of their largest, in `ranges`), a row of q to below
-// 2^15 after it has taken the keys' powers back. score_scale: what the products
-// of a row's scores are multiplied by, `scale` log2(e) and those powers.
+// [sequences][table_width]: whichever needs room for fewer. fp16 keeps 11 bits of
+// numbers from 2^-14 to 2^16 only, so all of it is scaled by powers of two: the
+// keys and the values of a head's 64 features to below 2^15 (half_shift() of their
+// largest, in `ranges`), a row of q to below 2^15 after it has taken the keys'
+// powers back. score_scale: what the products of a row's scores are multiplied by,
+// `scale` log2(e) and those powers.
 struct CacheUnpackArgs
 {
     CacheMemory mem;
