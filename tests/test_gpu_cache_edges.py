@@ -442,3 +442,26 @@ def test_lengths_that_change_behind_a_call(rows, storage):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     awa_b200.device_status()
+
+
+@pytest.mark.parametrize("window", [0, 60])
+@pytest.mark.parametrize("storage", ["bf16", "f32", "int4"])
+def test_many_rows_with_a_page_that_is_not_there(storage, window):
+    """Its rows are zeros to the attention, keys and values, and are reported."""
+    dtype = torch.float32 if storage == "f32" else torch.bfloat16
+    c = Batch([90], [200], 16, 2, 64, storage, seed=38)
+    real = c.table[0, 14].item()
+    c.table[0, 14] = -5
+    cache, batch = c.handles(awa_b200)
+    q = c.new_rows(8, dtype)
+    got = cache.attention(batch, q, sinks=4, window=window)
+    with pytest.raises(awa_b200.AwaError, match="71"):
+        awa_b200.device_status()
+    c.table[0, 14] = real
+    for t in ((c.k, c.v) if storage != "int4" else c.params):
+        t[real] = 0
+    if storage == "int4":
+        want, tol = four_bit_attention(c, q, 4, window, 1, 64 ** -0.5, True)
+    else:
+        want, tol = attention(c, q, 4, window, 1, 64 ** -0.5)
+    assert ((got.double() - want).abs() <= tol).all()
